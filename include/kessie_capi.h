@@ -556,6 +556,108 @@ int kessie_paged_fog_decode_cp_v2(const void* q, int64_t q_stride_b, int64_t q_s
                                   void* out, float* out_partial, void* workspace,
                                   size_t workspace_bytes, int phases, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* One scheduler step over the paged cache (no reference counterpart)        */
+/* ------------------------------------------------------------------------- */
+
+/* Page tables and slot maps of a step, from the requests' lengths, in one
+ * launch.  Request r has context_lens[r] cached and query_lens[r] new tokens
+ * (int32 [num_requests], num_requests <= 8192).  Its first
+ * ceil(context / page_size) pages are in block_table[r] (int32 rows of
+ * max_pages entries, block_table_stride apart); the pages it still needs are
+ * taken from the end of free_pages (int32 [num_free_pages]; only the first
+ * *free_count of them when free_count, a device int32, is given) in request
+ * order -- the batch's j-th new page is free_pages[F - 1 - j], the order
+ * KeSSiePagedKVCache.allocate_pages pops (kessie_hip_kernels.py:520-524) --
+ * and written into block_table.  Outputs:
+ *   query_start_loc int32 [num_requests + 1], seq_lens int32 [num_requests],
+ *   positions int32 and slot_mapping int64 [num_tokens]: of the batch's new
+ *   tokens in request order; slot = page * page_size + position % page_size;
+ *   rows past the last token (a padded batch) get position 0 and slot -1;
+ *   pages_used int32 [1]: entries taken from free_pages (free_pages itself
+ *   and free_count are not changed).
+ * KESSIE_DEV_BAD_ARG is recorded for a negative length (taken as 0), a
+ * sequence past the table's width, more tokens than num_tokens, or more pages
+ * than are free (table entries -1); KESSIE_DEV_BAD_PAGE_ID for a page id
+ * outside [0, num_pages).  The slots of the tokens concerned are -1. */
+int kessie_step_tables_v2(const int32_t* context_lens, const int32_t* query_lens, int num_requests,
+                          int32_t* block_table, int64_t block_table_stride, int max_pages,
+                          int page_size, int num_pages, const int32_t* free_pages,
+                          int num_free_pages, const int32_t* free_count, int num_tokens,
+                          int32_t* query_start_loc, int32_t* seq_lens, int32_t* positions,
+                          int64_t* slot_mapping, int32_t* pages_used, void* stream);
+
+/* Rotary embedding with one position per axis and token (time, height, width).
+ * sections (HOST int [num_axes], num_axes <= 8) gives each axis its number of
+ * the half = sum(sections) <= 256 frequencies f_d = theta^(-d / half) (fp32):
+ * in blocks (interleaved 0), or frequency d to axis d % num_axes while
+ * d < num_axes * sections[axis], else to axis 0 (interleaved 1; sections that
+ * this does not fill are refused).  Pairs (d, d + half) are turned by
+ * (target - orig)[axis(d)] * f_d, computed exactly (fixed-point turns);
+ * dimensions from 2 * half on pass through.  Positions int32
+ * [num_axes][num_tokens], rows *_axis_stride apart.
+ *
+ * remap: stored keys k [T, H, D] to out (out == k with k's strides: in place;
+ * otherwise they must not overlap); orig_positions NULL means 0. */
+int kessie_rope_axes_remap_v2(const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                              void* out, int64_t out_token_stride, int64_t out_head_stride,
+                              int dtype, int num_tokens, int num_heads, int head_dim,
+                              const int32_t* orig_positions, int64_t orig_axis_stride,
+                              const int32_t* target_positions, int64_t target_axis_stride,
+                              const int* sections, int num_axes, int interleaved,
+                              float rope_theta, void* stream);
+
+/* insert: the new tokens of a step.  q [T, Hq, D] turned into out_q (may be q
+ * itself), k [T, Hkv, D] turned and v copied into the cache rows named by
+ * slot_mapping (int64 [T]; page slot / page_size, token slot % page_size;
+ * negative: k and v are not written).  Slots must be distinct; one past the
+ * cache is skipped and records KESSIE_DEV_BAD_PAGE_ID.  kv_cache is addressed
+ * as in kessie_page_insert_v2. */
+int kessie_rope_axes_insert_v2(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                               void* out_q, int64_t out_token_stride, int64_t out_head_stride,
+                               const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                               const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                               int dtype, int num_tokens, int num_q_heads, int num_kv_heads,
+                               int head_dim, const int32_t* positions,
+                               int64_t positions_axis_stride, const int* sections, int num_axes,
+                               int interleaved, float rope_theta, void* kv_cache,
+                               int64_t page_stride, int64_t token_stride, int64_t kv_stride,
+                               int64_t head_stride, int num_pages, int page_size,
+                               const int64_t* slot_mapping, void* stream);
+
+/* Attention of ragged chunks over a paged cache: the new tokens of a whole
+ * step (decodes and prompt chunks mixed), without reading a length back to the
+ * host.  q and out [num_tokens, Hq, D] (f16 / bf16, D 64 or 128, Hq/Hkv <=
+ * 128, rows 16-byte aligned); rows query_start_loc[b] .. query_start_loc[b+1)
+ * (int32 [batch + 1]) belong to sequence b, the last of them at position
+ * seq_lens[b] - 1.  Keys j < min(seq_lens[b], max_seq_len) of block_table[b]
+ * are seen when j <= position (is_causal or a window) and
+ * position - j < window_size (window_size > 0); is_causal 0 without a window
+ * attends to all keys of another sequence (cross attention).
+ * Fog: clear_start / fog_alpha as in the decode (on V), or bias (added to the
+ * scaled scores, by key position, kv_len = the sequence's keys); both nullable.
+ * Rows that see no key are 0; rows of no sequence (a padded batch) are left as
+ * they were.  Keys that no row of a sequence sees are never used, so their
+ * pages may hold anything; keys that some of its rows see must be finite.
+ * A page id outside [0, num_pages) reads as zero keys and values and records
+ * KESSIE_DEV_BAD_PAGE_ID; a length past max_seq_len, or offsets that leave
+ * [0, num_tokens] or fall, are cut and record KESSIE_DEV_BAD_ARG.
+ * workspace: kessie_paged_fog_chunks_workspace_size() bytes, 16-byte aligned,
+ * no initialisation; calls that can overlap need one each. */
+size_t kessie_paged_fog_chunks_workspace_size(int num_q_heads, int num_kv_heads, int head_dim);
+int kessie_paged_fog_chunks_v2(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                               const void* k_cache, const void* v_cache, int64_t page_stride,
+                               int64_t token_stride, int64_t head_stride, int num_pages,
+                               int page_size, const int32_t* block_table,
+                               int64_t block_table_stride, const int32_t* query_start_loc,
+                               const int32_t* seq_lens, const int32_t* clear_start,
+                               float fog_alpha, int window_size, int is_causal, float sm_scale,
+                               int batch, int num_tokens, int num_q_heads, int num_kv_heads,
+                               int head_dim, int max_seq_len, int dtype,
+                               const kessie_fog_bias* bias, void* out, int64_t o_stride_t,
+                               int64_t o_stride_h, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

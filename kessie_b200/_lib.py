@@ -108,6 +108,17 @@ SIGNATURES = {
                                               I32P, c_int64, I32P, I32P, I32P, I32P, c_float, P, c_int, c_float,
                                               c_int, c_int, c_int, c_int, c_int, c_int, P, c_int, c_int, c_uint32,
                                               c_int64, P, P, P, c_size_t, c_int, P]),
+    "kessie_step_tables_v2": (c_int, [I32P, I32P, c_int, I32P, c_int64, c_int, c_int, c_int, I32P, c_int, I32P, c_int,
+                                      I32P, I32P, I32P, P, I32P, P]),
+    "kessie_rope_axes_remap_v2": (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, c_int, c_int, c_int, c_int, I32P,
+                                          c_int64, I32P, c_int64, P, c_int, c_int, c_float, P]),
+    "kessie_rope_axes_insert_v2": (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64,
+                                           c_int64, c_int, c_int, c_int, c_int, c_int, I32P, c_int64, P, c_int, c_int,
+                                           c_float, P, c_int64, c_int64, c_int64, c_int64, c_int, c_int, P, P]),
+    "kessie_paged_fog_chunks_workspace_size": (c_size_t, [c_int, c_int, c_int]),
+    "kessie_paged_fog_chunks_v2": (c_int, [P, c_int64, c_int64, P, P, c_int64, c_int64, c_int64, c_int, c_int, I32P,
+                                           c_int64, I32P, I32P, I32P, c_float, c_int, c_int, c_float, c_int, c_int,
+                                           c_int, c_int, c_int, c_int, c_int, P, P, c_int64, c_int64, P, c_size_t, P]),
 }
 
 _lock = threading.Lock()

@@ -14,7 +14,7 @@ from __future__ import annotations
 import ctypes
 import math
 import threading
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -81,6 +81,21 @@ def workspace(nbytes: int, device, tag: str = "default") -> torch.Tensor:
             buf = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
             _ws_cache[key] = buf
         return buf
+
+
+def _stream_workspace(nbytes: int, dev: torch.device, tag: str, handle: int) -> torch.Tensor:
+    """Scratch for a call on stream `handle` of `dev`: one buffer per stream,
+    so calls on two streams never share one; a capture gets a buffer of its
+    graph's memory pool, so two captured graphs may run at once.  `dev` is the
+    current device."""
+    current = _stream(None, dev.index)
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
+    if handle == current:
+        return workspace(nbytes, dev, f"{tag}@{handle}")
+    # allocated under the stream that uses it: the allocator hands memory out in that stream's order
+    with torch.cuda.stream(torch.cuda.ExternalStream(handle, device=dev)):
+        return workspace(nbytes, dev, f"{tag}@{handle}")
 
 
 def read_device_status(stream=None) -> int:
@@ -539,6 +554,237 @@ def paged_fog_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         B, T, Hq, Hkv, D, dtype_code(q), out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), mkv, ws_ptr,
         ws_n, _stream(stream)), "paged_fog_prefill")
     return out
+
+
+# --------------------------------------------------------------------- one scheduler step
+class StepTables(NamedTuple):
+    """What ``step_tables`` builds for a step (all on the device)."""
+    query_start_loc: torch.Tensor    # int32 [R + 1]
+    seq_lens: torch.Tensor           # int32 [R]
+    positions: torch.Tensor          # int32 [num_tokens]
+    slot_mapping: torch.Tensor       # int64 [num_tokens], -1 past the last token
+    pages_used: torch.Tensor         # int32 [1]
+
+
+def _same_device(name: str, dev: torch.device, *ts):
+    for t in ts:
+        if torch.is_tensor(t) and t.device != dev:
+            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
+
+
+def _step_output(name: str, t: Optional[torch.Tensor], n: int, dtype, device) -> torch.Tensor:
+    if t is None:
+        return torch.empty(n, dtype=dtype, device=device)
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"step_tables: {name} must be a contiguous {dtype} tensor of {n} elements")
+    return t
+
+
+def step_tables(context_lens: torch.Tensor, query_lens: torch.Tensor, block_table: torch.Tensor, page_size: int,
+                free_pages: torch.Tensor, num_tokens: int, num_pages: Optional[int] = None,
+                free_count: Optional[torch.Tensor] = None, out: Optional["StepTables"] = None,
+                stream=None) -> "StepTables":
+    """Page tables and slot maps of one scheduler step from the requests'
+    lengths, in one launch and without a host read.
+
+    Request r has context_lens[r] cached and query_lens[r] new tokens; the
+    first ceil(context / page_size) entries of block_table[r] (int32 [R,
+    maxP], entries contiguous) are its pages.  The pages its new tokens need
+    are popped from the end of free_pages (int32 [F]; of its first
+    free_count[0] when that device tensor is given), in request order, and
+    written into block_table.  num_tokens is the size of the per-token outputs
+    (the batch's new tokens, or the padded size of a captured batch: rows past
+    the last token get position 0 and slot -1).  num_pages (the pool's size)
+    bounds the page ids.  `out` reuses an earlier result's tensors.  Lengths
+    that do not fit are cut and recorded in the device status
+    (read_device_status), with -1 for the pages and slots concerned."""
+    _need_cuda(context_lens, query_lens, block_table, free_pages, free_count)
+    dev = block_table.device
+    _same_device("step_tables", dev, context_lens, query_lens, free_pages, free_count, *(out or ()))
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
+            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("step_tables: block_table must be int32 [R, maxP] with contiguous rows (it is updated in place)")
+    R = block_table.shape[0]
+    if context_lens.numel() != R or query_lens.numel() != R:
+        raise ValueError("step_tables: one context and one query length per row of block_table")
+    ctx, new, free = (_i32(t, dev) for t in (context_lens, query_lens, free_pages))
+    if free_count is not None:
+        if free_count.numel() != 1:
+            raise ValueError("step_tables: free_count has one element")
+        free_count = _i32(free_count, dev)
+    shapes = (("query_start_loc", R + 1, torch.int32), ("seq_lens", R, torch.int32),
+              ("positions", int(num_tokens), torch.int32), ("slot_mapping", int(num_tokens), torch.int64),
+              ("pages_used", 1, torch.int32))
+    if num_tokens < 0:
+        raise ValueError("step_tables: num_tokens must not be negative")
+    res = StepTables(*(_step_output(name, getattr(out, name) if out is not None else None, n, dt, dev)
+                       for name, n, dt in shapes))
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().kessie_step_tables_v2(
+            _p(ctx), _p(new), R, _p(block_table), block_table.stride(0), block_table.shape[1], int(page_size),
+            2 ** 31 - 1 if num_pages is None else int(num_pages), _p(free), free.numel(), _p(free_count),
+            int(num_tokens), *(_p(t) for t in res), _stream(stream, dev.index)), "step_tables")
+    return res
+
+
+def _axis_positions(name: str, positions, axes: int, tokens: int, device) -> torch.Tensor:
+    t = positions if torch.is_tensor(positions) else torch.as_tensor(positions, device=device)
+    if t.dim() == 1 and axes == 1:
+        t = t.unsqueeze(0)
+    if t.shape != (axes, tokens):
+        raise ValueError(f"{name}: positions must be [{axes}, {tokens}], one row per axis, got {tuple(t.shape)}")
+    _need_cuda(t)
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    return t if t.stride(1) == 1 or tokens <= 1 else t.contiguous()
+
+
+def _sections(name: str, sections: Sequence[int]):
+    sec = [int(x) for x in sections]
+    if not sec:
+        raise ValueError(f"{name}: sections must give each axis its number of frequencies")
+    return (ctypes.c_int * len(sec))(*sec), len(sec)
+
+
+def _rows(name: str, x: torch.Tensor):
+    if x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
+        raise ValueError(f"{name}: rows must be [tokens, heads, head_dim] with head_dim contiguous")
+    return x.stride(0), x.stride(1)
+
+
+def rope_axes_remap(k: torch.Tensor, orig_positions, target_positions, sections: Sequence[int],
+                    rope_theta: float = 10000.0, interleaved: bool = False, out: Optional[torch.Tensor] = None,
+                    stream=None) -> torch.Tensor:
+    """Re-rotate keys [T, H, D] whose rotary embedding has one position per
+    axis (rope_remap's form for image and video tokens), in place or into
+    `out`.  orig_positions / target_positions: int32 [axes, T]; sections: the
+    number of frequencies of each axis, sum(sections) = half the rotated
+    dimensions; in blocks, or interleaved over the frequencies (d to axis
+    d % axes while d < axes * sections[axis], else to the first).  With
+    orig_positions None the keys are rotated from position 0.  Angles are
+    exact to fp32 at any int32 position."""
+    _need_cuda(k, out)
+    out = k if out is None else out
+    if out.shape != k.shape or out.dtype != k.dtype:
+        raise ValueError("rope_axes_remap: out must match k's shape and dtype")
+    T, H, D = k.shape
+    ks, os_ = _rows("rope_axes_remap", k), _rows("rope_axes_remap", out)
+    sec, axes = _sections("rope_axes_remap", sections)
+    tgt = _axis_positions("rope_axes_remap", target_positions, axes, T, k.device)
+    org = None if orig_positions is None else _axis_positions("rope_axes_remap", orig_positions, axes, T, k.device)
+    _same_device("rope_axes_remap", k.device, out, tgt, org)
+    with torch.cuda.device(k.device):
+        _lib.check(_lib.load().kessie_rope_axes_remap_v2(
+            _p(k), *ks, _p(out), *os_, dtype_code(k), T, H, D, _p(org), org.stride(0) if org is not None else 0,
+            _p(tgt), tgt.stride(0), sec, axes, 1 if interleaved else 0, float(rope_theta),
+            _stream(stream, k.device.index)), "rope_axes_remap")
+    return out
+
+
+def rope_axes_insert(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions, sections: Sequence[int],
+                     kv: torch.Tensor, slot_mapping: torch.Tensor, rope_theta: float = 10000.0,
+                     interleaved: bool = False, out_q: Optional[torch.Tensor] = None, layout: str = "kessie",
+                     stream=None) -> torch.Tensor:
+    """The new tokens of a step, before the attention: rotate q [T, Hq, D]
+    (in place or into out_q; returned) and k [T, Hkv, D] by positions [axes,
+    T], and write k and v [T, Hkv, D] to the rows of the paged cache `kv`
+    (layout as in page_insert) that slot_mapping (int64 [T], page * page_size +
+    token; negative: not written) names.  Sections and angles as in
+    rope_axes_remap; slots must be distinct.  One launch."""
+    _need_cuda(q, k, v, kv, slot_mapping, out_q)
+    out_q = q if out_q is None else out_q
+    T, Hq, D = q.shape
+    ps_, ts_, kvs_, hs_, P, ps, Hkv, Dc = kv_layout_strides(kv, layout)
+    if k.shape != (T, Hkv, D) or v.shape != k.shape or Dc != D or out_q.shape != q.shape:
+        raise ValueError(f"rope_axes_insert: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, "
+                         f"out_q {tuple(out_q.shape)} do not match a cache of {Hkv} heads of {Dc}")
+    if not (q.dtype == k.dtype == v.dtype == kv.dtype == out_q.dtype):
+        raise TypeError("rope_axes_insert: q, k, v, out_q and the cache share one dtype")
+    if kv.stride(-1) != 1:
+        raise ValueError("rope_axes_insert: the cache's head_dim must be contiguous")
+    if slot_mapping.numel() != T:
+        raise ValueError("rope_axes_insert: slot_mapping has one entry per token")
+    qs, ks, vs, os_ = (_rows("rope_axes_insert", x) for x in (q, k, v, out_q))
+    sec, axes = _sections("rope_axes_insert", sections)
+    pos = _axis_positions("rope_axes_insert", positions, axes, T, q.device)
+    _same_device("rope_axes_insert", q.device, k, v, kv, slot_mapping, out_q, pos)
+    slots = slot_mapping.to(torch.int64).contiguous()
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.load().kessie_rope_axes_insert_v2(
+            _p(q), *qs, _p(out_q), *os_, _p(k), *ks, _p(v), *vs, dtype_code(q), T, Hq, Hkv, D, _p(pos), pos.stride(0),
+            sec, axes, 1 if interleaved else 0, float(rope_theta), _p(kv), ps_, ts_, kvs_, hs_, P, ps, _p(slots),
+            _stream(stream, q.device.index)), "rope_axes_insert")
+    return out_q
+
+
+def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                     query_start_loc: torch.Tensor, seq_lens: torch.Tensor, clear_start=None, fog_alpha: float = 0.5,
+                     window_size: int = 0, causal: bool = True, sm_scale: Optional[float] = None,
+                     max_seq_len: Optional[int] = None, out: Optional[torch.Tensor] = None, stream=None,
+                     ws: Optional[torch.Tensor] = None, bias: Optional["FogBias"] = None) -> torch.Tensor:
+    """Fog attention of ragged chunks of new tokens over a paged cache: a
+    step's decodes and prompt chunks in one call, no length read by the host
+    (paged_fog_decode is the form for one token each, paged_fog_prefill for
+    chunks of one length).
+
+    q [T, Hq, D] (f16 / bf16): rows query_start_loc[b] .. query_start_loc[b+1)
+    (int32 [B + 1]) are sequence b's new tokens, the last one at position
+    seq_lens[b] - 1 (seq_lens counts them); k_cache / v_cache [P, ps, Hkv, D]
+    views, block_table [B, maxP].  causal=False without a window attends to
+    all of the sequence's keys, whatever the number of queries (cross
+    attention).  clear_start / fog_alpha or bias as in paged_fog_decode.
+    Returns out [T, Hq, D]; rows that see no key are 0, rows of no sequence (a
+    padded batch) are not written.  Scratch memory: one buffer per stream, a
+    graph capture gets its own; or `ws` (chunks_workspace_bytes() bytes)."""
+    _need_cuda(q, k_cache, v_cache, block_table, query_start_loc, seq_lens, out)
+    T, Hq, D = q.shape
+    P, ps, Hkv, Dk = k_cache.shape
+    ks = k_cache.stride()
+    if Dk != D or v_cache.shape != k_cache.shape or v_cache.stride() != ks:
+        raise ValueError("k_cache/v_cache must be matching [P, ps, Hkv, D] views")
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise TypeError("q and the cache must share a dtype")
+    if ks[3] != 1:
+        raise ValueError("head_dim must be contiguous")
+    B = block_table.shape[0]
+    if query_start_loc.numel() != B + 1 or seq_lens.numel() != B:
+        raise ValueError("paged_fog_chunks: block_table [B, maxP], query_start_loc [B + 1], seq_lens [B]")
+    if q.stride(2) != 1 or (q.stride(0) | q.stride(1)) % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)      # rows the kernel cannot load: a copy
+    if out is None:
+        out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError("paged_fog_chunks: out must match q, head_dim contiguous")
+    dev = q.device
+    bt = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
+    if bt.stride(1) != 1:
+        bt = bt.contiguous()
+    qsl, sl, cs = _i32(query_start_loc, dev), _i32(seq_lens, dev), _i32(clear_start, dev)
+    _same_device("paged_fog_chunks", dev, k_cache, v_cache, bt, qsl, sl, cs, out)
+    cap = bt.shape[1] * ps
+    if max_seq_len is None:
+        max_seq_len = cap
+    if max_seq_len > cap:
+        raise ValueError(f"max_seq_len {max_seq_len} exceeds the block table capacity {cap}")
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(D)
+    lib = _lib.load()
+    cb = bias.c_struct() if bias is not None else None
+    with torch.cuda.device(dev):
+        handle = _stream(stream, dev.index)
+        if ws is None:
+            ws = _stream_workspace(lib.kessie_paged_fog_chunks_workspace_size(Hq, Hkv, D), dev, "chunks", handle)
+        _lib.check(lib.kessie_paged_fog_chunks_v2(
+            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], P, ps,
+            bt.data_ptr(), bt.stride(0), qsl.data_ptr(), sl.data_ptr(), _p(cs), float(fog_alpha), int(window_size),
+            1 if causal else 0, float(sm_scale), B, T, Hq, Hkv, D, int(max_seq_len), dtype_code(q),
+            ctypes.byref(cb) if cb is not None else None, out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr(),
+            ws.numel(), handle), "paged_fog_chunks")
+    return out
+
+
+def chunks_workspace_bytes(num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    return int(_lib.load().kessie_paged_fog_chunks_workspace_size(num_q_heads, num_kv_heads, head_dim))
 
 
 # --------------------------------------------------------------------- conversation index
