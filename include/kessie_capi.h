@@ -630,12 +630,13 @@ int kessie_rope_axes_insert_v2(const void* q, int64_t q_token_stride, int64_t q_
  * host.  q and out [num_tokens, Hq, D] (f16 / bf16, D 64 or 128, Hq/Hkv <=
  * 128, rows 16-byte aligned); rows query_start_loc[b] .. query_start_loc[b+1)
  * (int32 [batch + 1]) belong to sequence b, the last of them at position
- * seq_lens[b] - 1.  Keys j < min(seq_lens[b], max_seq_len) of block_table[b]
- * are seen when j <= position (is_causal or a window) and
+ * seq_lens[b] - 1 (batch <= 8192).  Keys j < min(seq_lens[b], max_seq_len) of
+ * block_table[b] (max_seq_len within the table's rows) are seen when j <= position (is_causal or a window) and
  * position - j < window_size (window_size > 0); is_causal 0 without a window
  * attends to all keys of another sequence (cross attention).
  * Fog: clear_start / fog_alpha as in the decode (on V), or bias (added to the
- * scaled scores, by key position, kv_len = the sequence's keys); both nullable.
+ * scaled scores, by key position, kv_len = the sequence's keys); both nullable,
+ * not both at once.
  * Rows that see no key are 0; rows of no sequence (a padded batch) are left as
  * they were.  Keys that no row of a sequence sees are never used, so their
  * pages may hold anything; keys that some of its rows see must be finite.

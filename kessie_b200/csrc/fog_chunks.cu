@@ -1,5 +1,6 @@
 // fog_chunks.cu -- attention of ragged chunks of new tokens over a paged KV
-// cache (one launch for a whole mixed batch of decodes and prompt chunks).
+// cache: a whole mixed batch of decodes and prompt chunks, planned on the
+// device, on the 5th-generation tensor cores.
 //
 // Query row t of sequence b (rows query_start_loc[b] .. [b + 1) of q) sits at
 // position seq_lens[b] - n_b + t and sees the keys j < seq_lens[b] with
@@ -9,10 +10,41 @@
 // (kessie_hip_kernels.py:403-413,577-593) or the additive fog bias
 // (kessie_attention.py:114-139).  A row that sees no key is 0.
 //
-// First form: one warp per (query row, head), one key at a time.
+// Tiles.  Rows are (token, head-in-group) pairs of one KV head, so the G query
+// heads that share a KV head share every K/V tile.  TH = 128 / G tokens make
+// one 128-row half; a tile is two halves A, B (a "pair" tile: both read each
+// 128-key tile) or, when its tokens fit one half (decodes, short chunks), a
+// "single" tile: the same rows twice, A over the even and B over the odd key
+// tiles, merged at the end.  Either way two independent score / softmax /
+// product chains alternate on the tensor core.
+//
+// Plan.  The key tiles of all (sequence, KV head, tile) triples are laid end
+// to end, each weighted with what it costs (kCostPair / kCostSingle per key
+// tile, kCostTile per tile), and the persistent grid's CTA c streams the
+// equal range [c L, (c + 1) L): no wave quantisation, whatever the mix of
+// lengths.  Every CTA derives the plan itself from the length arrays.  A tile
+// cut by a range boundary leaves fp32 partials (O, m, l) of each piece in the
+// workspace, at most two a CTA, and fog_chunks_merge_kernel joins them in
+// order, so results do not depend on timing.
+//
+// CTA = 12 warps: 0-3 / 4-7 softmax of A / B (one row per thread: TMEM lane =
+// row), 8 Q and K producer, 9 MMA issuer (one thread) and TMEM owner, 10 V
+// producer, 11 fog weights.  TMEM columns: S_A [0,128) S_B [128,256) O_A
+// [256,..) O_B [384,..); P (16-bit pairs) overwrites the first 64 columns of
+// its S.  Per event e (alternating A, B): wait P(e), O += P V, then S(e + 2) =
+// Q K^T into the region P(e) left, so one chain's MMAs run under the other's
+// softmax.  Producers run ahead over tile ends.
+//
+// K/V come straight from the pages: one TMA box per page (up to 128 tokens)
+// lands as [token / 8][D / 64][8][64] with 128-byte swizzle, whose 8-row groups
+// have one stride, so a K or V tile of any page size is one matrix operand.
+//
+// Every mbarrier wait is bounded; on a timeout all warps still reach the final
+// barrier and the TMEM is freed.
 #include "common.cuh"
 #include "fog_bias.cuh"
 #include "ptx.cuh"
+#include "tma_host.cuh"
 
 #include <limits.h>
 #include <math.h>
@@ -20,62 +52,838 @@
 namespace kessie {
 namespace {
 
+constexpr int kThreads = 384;
+constexpr int kSoftmaxWarps = 8;
+constexpr int kMaxBatch = 8192;              // sequences whose prefix sums the plan keeps in shared memory
+constexpr int kWStages = 4;                  // key tiles of fog weights in flight
+constexpr uint32_t kTmemCols = 512;
+constexpr float kRescaleThreshold = 8.0f;    // log2 units the running max may lag behind
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kProducerRegs = 64;
+static_assert(256 * kSoftmaxRegs + 128 * kProducerRegs <= kThreads * kLaunchRegs, "register split exceeds the pool");
+
+// Plan weights of a 128-key tile (pair / single) and of starting and ending a tile.
+constexpr int kCostPair = 3, kCostSingle = 2, kCostTile = 4;
+
+enum FogMode { kNoFog = 0, kValueFog = 1, kScoreFog = 2 };
+
 struct ChunkParams {
-    const void* q; int64_t q_st, q_sh;
     void* o; int64_t o_st, o_sh;
-    const void* k; const void* v;
-    int64_t page_stride, token_stride, head_stride;
     int num_pages, page_size;
     const int32_t* table; int64_t table_stride;
     const int32_t* start; const int32_t* seq;
     const int32_t* clear_start; float fog_alpha;
     int window, causal;
-    float scale;
-    int B, T, Hq, Hkv, G, max_seq;
+    float scale_log2;
+    int B, T, Hkv, G, TH, max_seq;
     FogBias bias;
     int* status;
+    // K/V boxes: tokens per box, page coordinate = page * page_mul + head * head_in_page, third coordinate =
+    // head * head_in_row; split: one box per 64 dims into separate half tiles
+    int box, page_mul, head_in_page, head_in_row, split;
+    int oob_page;                            // page coordinate that reads zeros
+    char* ws;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128) fog_chunks_simple_kernel(const ChunkParams p) {
-    const int b = blockIdx.y, lane = threadIdx.x & 31;
-    const int h = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (h >= p.Hq) return;
-    const int s0 = p.start[b], s1 = p.start[b + 1];
-    const int r0 = min(max(s0, 0), p.T), r1 = max(r0, min(s1, p.T));
-    const int len = p.seq[b];
-    const int kv = min(max(len, 0), p.max_seq);
-    if (r0 != s0 || r1 != s1 || kv != len) record_status(p.status, KESSIE_DEV_BAD_ARG);
-    const int cs = p.clear_start && p.fog_alpha > 0.f ? p.clear_start[b] : INT_MIN;
-    const int fb = p.bias.on ? fog_bias_boundary(p.bias, kv) : 0;
-    constexpr int N = D / 32;
-    for (int t = r0; t < r1; ++t) {
-        const int pos = len - (r1 - r0) + (t - r0);
-        const int hi = (p.causal || p.window > 0) ? min(kv, pos + 1) : kv;
-        const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-        const T* q = static_cast<const T*>(p.q) + t * p.q_st + h * p.q_sh + lane * N;
-        float qr[N], acc[N], m = -INFINITY, l = 0.f;
-        for (int i = 0; i < N; ++i) { qr[i] = to_f32(q[i]) * p.scale; acc[i] = 0.f; }
-        for (int j = lo; j < hi; ++j) {
-            const int id = p.table[b * p.table_stride + j / p.page_size];
-            const bool ok = id >= 0 && id < p.num_pages;
-            if (!ok) record_status(p.status, KESSIE_DEV_BAD_PAGE_ID);
-            const int64_t off = (int64_t)(ok ? id : 0) * p.page_stride + (j % p.page_size) * p.token_stride +
-                                (h / p.G) * p.head_stride + lane * N;
-            float s = 0.f;
-            for (int i = 0; i < N; ++i) s += ok ? qr[i] * to_f32(static_cast<const T*>(p.k)[off + i]) : 0.f;
-            for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-            if (p.bias.on) s += fog_bias_at(p.bias, fb, j);
-            const float m_new = fmaxf(m, s), f = expf(m - m_new), e = expf(s - m_new);
-            const float w = j < cs ? powf((float)j / (float)max(cs - 1, 1), p.fog_alpha) : 1.f;
-            l = l * f + e;
-            m = m_new;
-            for (int i = 0; i < N; ++i)
-                acc[i] = acc[i] * f + (ok ? e * w * to_f32(static_cast<const T*>(p.v)[off + i]) : 0.f);
-        }
-        T* o = static_cast<T*>(p.o) + t * p.o_st + h * p.o_sh + lane * N;
-        for (int i = 0; i < N; ++i) o[i] = from_f32<T>(l > 0.f ? acc[i] / l : 0.f);
+template <int D> struct Cfg {
+    static constexpr int DH = D / 64;
+    static constexpr int kTile = 128 * D * 2;          // one K, V or Q half tile
+    static constexpr int kNK = D == 128 ? 2 : 4;
+    static constexpr int kNV = D == 128 ? 2 : 4;
+    static constexpr int kQ = 0;                       // two half slots
+    static constexpr int kK = 2 * kTile;
+    static constexpr int kV = kK + kNK * kTile;
+    static constexpr int kW = kV + kNV * kTile;        // fog weights
+    static constexpr int kMl = kW + kWStages * 128 * 4;    // (m, l) of a single tile's B chain
+    static constexpr int kBar = kMl + 128 * 8;
+    static constexpr int kNumBar = 4 + 2 * kNK + 2 * kNV + 2 * kWStages + 2 + 2 + 2 + 2;
+    static constexpr int kPlan = kBar + kNumBar * 8;   // plan result and TMEM slot
+    static constexpr int kBytes = kPlan + 64;
+    static constexpr int kAlloc = kBytes + 1024;
+    static_assert(kNV * kTile >= kMaxBatch * 8, "the plan's prefix sums use the V ring");
+    // partial slot in the workspace: O float4 [D / 4][256 rows], (m, l) float2 [256]
+    static constexpr size_t kSlotBytes = (size_t)256 * D * 4 + 256 * 8;
+};
+
+// What the merge needs to know of CTA c's first piece.
+struct PieceDesc { int mid, ends, b, hk, tok0, ntok, row0, pad; };
+
+struct Seq { int n, q0, kv, row0; };
+
+__device__ __forceinline__ Seq load_seq(const ChunkParams& p, int b, bool* bad = nullptr) {
+    const int s0 = __ldg(p.start + b), s1 = __ldg(p.start + b + 1), len = __ldg(p.seq + b);
+    Seq s;
+    s.row0 = min(max(s0, 0), p.T);
+    const int e = max(s.row0, min(s1, p.T));
+    s.n = e - s.row0;
+    s.kv = min(max(len, 0), p.max_seq);
+    s.q0 = len - s.n;
+    if (bad && (s.row0 != s0 || e != s1 || s.kv != len)) *bad = true;
+    return s;
+}
+
+// Key range of tile i of a sequence: keys [j_lo, j_hi), key tiles [t_lo, t_hi) (at least one).
+struct TileKeys { int ntok, j_lo, j_hi, t_lo, t_hi; bool single; };
+
+__device__ __forceinline__ TileKeys tile_keys(const ChunkParams& p, const Seq& s, int i) {
+    TileKeys k;
+    const int tok0 = i * 2 * p.TH;
+    k.ntok = min(s.n - tok0, 2 * p.TH);
+    k.single = k.ntok <= p.TH;
+    const int p_lo = s.q0 + tok0, p_hi = p_lo + k.ntok - 1;
+    k.j_hi = (p.causal || p.window > 0) ? max(0, min(s.kv, p_hi + 1)) : s.kv;
+    k.j_lo = p.window > 0 ? min(max(p_lo - p.window + 1, 0), k.j_hi) : 0;
+    k.t_lo = k.j_lo >> 7;
+    k.t_hi = max(k.t_lo + 1, (k.j_hi + 127) >> 7);
+    return k;
+}
+__device__ __forceinline__ int tile_cost(const TileKeys& k) {
+    return (k.t_hi - k.t_lo) * (k.single ? kCostSingle : kCostPair) + kCostTile;
+}
+// Key tile of a tile's range at plan position x (relative to the tile's start).
+__device__ __forceinline__ int key_tile_at(const TileKeys& k, int64_t x) {
+    const int w = k.single ? kCostSingle : kCostPair;
+    const int64_t y = (x - kCostTile + w - 1);
+    return y <= 0 ? 0 : (int)min(y / w, (int64_t)(k.t_hi - k.t_lo));
+}
+
+struct Plan { int64_t u0, u1, pos; int b, hk, i, any; };
+
+// One piece of work: key tiles [k0, k1) of tile i of (b, hk).
+struct Item {
+    int b, hk, tok0, ntok, row0, q0, kv, j_lo, j_hi;
+    int key0;                 // first key of the piece's first key tile
+    int n;                    // key tiles
+    bool single, first, last; // one half; starts / ends with its tile
+};
+
+// Walks the pieces of this CTA's range; every warp role walks them alike.
+struct Walker {
+    const ChunkParams& p;
+    int64_t u0, u1, pos;
+    int b, hk, i;
+    Seq s;
+    bool more;
+    __device__ Walker(const ChunkParams& p_, const Plan& pl) : p(p_), u0(pl.u0), u1(pl.u1), pos(pl.pos), b(pl.b),
+                                                              hk(pl.hk), i(pl.i), more(pl.any != 0) {
+        if (more) s = load_seq(p, b);
     }
+    __device__ bool next(Item& it) {
+        while (more) {
+            const TileKeys k = tile_keys(p, s, i);
+            const int cost = tile_cost(k);
+            const int a = key_tile_at(k, u0 - pos), e = key_tile_at(k, u1 - pos);
+            it.b = b; it.hk = hk; it.tok0 = i * 2 * p.TH; it.ntok = k.ntok; it.row0 = s.row0 + it.tok0;
+            it.q0 = s.q0 + it.tok0; it.kv = s.kv; it.j_lo = k.j_lo; it.j_hi = k.j_hi;
+            it.key0 = (k.t_lo + a) << 7; it.n = e - a; it.single = k.single;
+            it.first = a == 0; it.last = e == k.t_hi - k.t_lo;
+            // on to the next tile
+            pos += cost;
+            if (pos >= u1) more = false;
+            else if ((i + 1) * 2 * p.TH < s.n) ++i;
+            else {
+                i = 0;
+                if (++hk == p.Hkv) {
+                    hk = 0;
+                    do {
+                        if (++b >= p.B) { more = false; break; }
+                        s = load_seq(p, b);
+                    } while (s.n == 0);
+                }
+            }
+            if (it.n > 0) return true;
+        }
+        return false;
+    }
+};
+
+// This CTA's range of the plan (all threads; `pre` is shared scratch for B prefix sums).
+__device__ __forceinline__ void make_plan(const ChunkParams& p, int64_t* pre, int64_t* wsum, Plan* out) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int64_t carry = 0;
+    bool bad = false;
+    const int TT = 2 * p.TH;
+    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+        const int b = b0 + tid;
+        Seq s{0, 0, 0, 0};
+        if (b < p.B) s = load_seq(p, b, &bad);
+        const int nt = (s.n + TT - 1) / TT;
+        int64_t c = 0;
+        if (nt <= 2)
+            for (int i = 0; i < nt; ++i) c += tile_cost(tile_keys(p, s, i));
+        // long sequences: the warp's lanes share the tiles
+        for (unsigned m = __ballot_sync(0xffffffffu, nt > 2); m; m &= m - 1) {
+            const int src = __ffs(m) - 1;
+            Seq t;
+            t.n = __shfl_sync(0xffffffffu, s.n, src);
+            t.q0 = __shfl_sync(0xffffffffu, s.q0, src);
+            t.kv = __shfl_sync(0xffffffffu, s.kv, src);
+            t.row0 = 0;
+            const int tn = (t.n + TT - 1) / TT;
+            int64_t x = 0;
+            for (int i = lane; i < tn; i += 32) x += tile_cost(tile_keys(p, t, i));
+#pragma unroll
+            for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+            if (lane == src) c = x;
+        }
+        c *= p.Hkv;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, c, d);
+            if (lane >= d) c += y;
+        }
+        if (lane == 31) wsum[warp] = c;
+        __syncthreads();
+        int64_t off = carry, all = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) off += wsum[w];
+            all += wsum[w];
+        }
+        if (b < p.B) pre[b] = off + c;
+        carry += all;
+        __syncthreads();
+    }
+    if (bad && blockIdx.x == 0) record_status(p.status, KESSIE_DEV_BAD_ARG);
+    if (warp == 0) {
+        const int64_t W = carry;
+        // a range holds at least one key tile, so no piece between two others is empty
+        const int64_t L = max((W + gridDim.x - 1) / (int64_t)gridDim.x, (int64_t)(kCostTile + 2 * kCostPair));
+        const int64_t u0 = blockIdx.x * L;
+        Plan pl{u0, min(u0 + L, W), 0, 0, 0, 0, u0 < W ? 1 : 0};
+        if (pl.any) {
+            int lo = 0, hi = p.B - 1;                       // first b with pre[b] > u0
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (pre[mid] > u0) hi = mid; else lo = mid + 1;
+            }
+            pl.b = lo;
+            const int64_t base = lo ? pre[lo - 1] : 0;
+            const int64_t per_head = (pre[lo] - base) / p.Hkv;
+            pl.hk = (int)((u0 - base) / per_head);
+            int64_t at = base + pl.hk * per_head;
+            const Seq s = load_seq(p, lo);
+            for (int i0 = 0;; i0 += 32) {
+                const int i = i0 + lane;
+                int64_t c = i * TT < s.n ? tile_cost(tile_keys(p, s, i)) : 0;
+                const int64_t own = c;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int64_t y = __shfl_up_sync(0xffffffffu, c, d);
+                    if (lane >= d) c += y;
+                }
+                const unsigned m = __ballot_sync(0xffffffffu, at + c > u0);
+                if (m) {
+                    const int src = __ffs(m) - 1;
+                    pl.i = i0 + src;
+                    pl.pos = at + __shfl_sync(0xffffffffu, c - own, src);
+                    break;
+                }
+                at += __shfl_sync(0xffffffffu, c, 31);
+                if ((i0 + 32) * TT >= s.n) { pl.any = 0; break; }      // not reached: the head holds u0
+            }
+        }
+        if (lane == 0) *out = pl;
+    }
+}
+
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, int n) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0], %1;\n\t}"
+                 :: "r"(ptx::smem_u32(bar)), "r"(n) : "memory");
+}
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity));
+}
+
+// Key tiles of a piece, from its first on, that need per-key weights.
+template <int FOG>
+__device__ __forceinline__ int fog_tiles(const ChunkParams& p, const Item& it, int edge) {
+    if (FOG == kNoFog) return 0;
+    if (FOG == kScoreFog && p.bias.recall) return it.n;
+    return min(it.n, max(0, (edge - it.key0 + 127) >> 7));
+}
+// First key past the fog of a sequence.
+template <int FOG>
+__device__ __forceinline__ int fog_edge(const ChunkParams& p, int b, int kv) {
+    if (FOG == kValueFog) return __ldg(p.clear_start + b);
+    if (FOG == kScoreFog) return fog_bias_boundary(p.bias, kv);
+    return 0;
+}
+
+// p = 2^(s * scale + nb) of one row's 128 scores, packed to 16-bit pairs over
+// the first 64 columns of the row's S; FOG == kValueFog with `wts`: p * w is
+// packed.  Returns the row sum of the unweighted, unrounded p.
+template <bool BF16, bool WEIGHTED>
+__device__ __forceinline__ float softmax_p(const uint32_t (&sv)[4][32], uint32_t sreg, float scale, float nb,
+                                           const float* wts) {
+    const uint64_t sc2 = ptx::f2_pack(scale, scale), nb2 = ptx::f2_pack(nb, nb);
+    uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint64_t s2 = ptx::f2_pack(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1]));
+            float e0, e1;
+            ptx::f2_unpack(ptx::ffma2(s2, sc2, nb2), e0, e1);
+            float p0 = ptx::ex2(e0), p1 = ptx::ex2(e1);
+            sum[i & 1] = ptx::fadd2(sum[i & 1], ptx::f2_pack(p0, p1));
+            if (WEIGHTED) {
+                const float2 w = *reinterpret_cast<const float2*>(wts + c * 32 + 2 * i);
+                p0 *= w.x;
+                p1 *= w.y;
+            }
+            pk[i] = ptx::pack2<BF16>(p0, p1);
+        }
+        ptx::tmem_st16(sreg + c * 16, pk);
+    }
+    ptx::tmem_st_wait();
+    float a0, a1, b0, b1;
+    ptx::f2_unpack(sum[0], a0, a1);
+    ptx::f2_unpack(sum[1], b0, b1);
+    return (a0 + a1) + (b0 + b1);
+}
+
+template <int D, bool BF16, int FOG>
+__global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_constant__ CUtensorMap tmQ,
+                                                                 const __grid_constant__ CUtensorMap tmK,
+                                                                 const __grid_constant__ CUtensorMap tmV,
+                                                                 const __grid_constant__ ChunkParams p) {
+    using C = Cfg<D>;
+    constexpr int DH = C::DH;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBar);
+    uint64_t* q_full = bars;                       // [2] half slots
+    uint64_t* q_empty = q_full + 2;
+    uint64_t* k_full = q_empty + 2;
+    uint64_t* k_empty = k_full + C::kNK;
+    uint64_t* v_full = k_empty + C::kNK;
+    uint64_t* v_empty = v_full + C::kNV;
+    uint64_t* w_full = v_empty + C::kNV;
+    uint64_t* w_empty = w_full + kWStages;
+    uint64_t* s_full = w_empty + kWStages;         // [2] chains A, B
+    uint64_t* p_full = s_full + 2;
+    uint64_t* o_full = p_full + 2;
+    uint64_t* o_free = o_full + 2;                 // every softmax warp is done with the piece's O
+    uint64_t* ml_full = o_free + 1;                // B's (m, l) of a single tile
+    Plan* plan = reinterpret_cast<Plan*>(smem + C::kPlan);
+    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::kPlan + 48);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&q_full[i], 1); ptx::mbar_init(&q_empty[i], 1);
+            ptx::mbar_init(&s_full[i], 1); ptx::mbar_init(&p_full[i], 4); ptx::mbar_init(&o_full[i], 1);
+        }
+        for (int i = 0; i < C::kNK; ++i) { ptx::mbar_init(&k_full[i], 1); ptx::mbar_init(&k_empty[i], 1); }
+        for (int i = 0; i < C::kNV; ++i) { ptx::mbar_init(&v_full[i], 1); ptx::mbar_init(&v_empty[i], 1); }
+        for (int i = 0; i < kWStages; ++i) { ptx::mbar_init(&w_full[i], 1); ptx::mbar_init(&w_empty[i], kSoftmaxWarps); }
+        ptx::mbar_init(o_free, kSoftmaxWarps);
+        ptx::mbar_init(ml_full, 4);
+        ptx::fence_mbar_init();
+    }
+    if (warp == 9) {
+        ptx::tmem_alloc(slot, kTmemCols);
+        ptx::tmem_relinquish();
+    }
+    make_plan(p, reinterpret_cast<int64_t*>(smem + C::kV), reinterpret_cast<int64_t*>(smem + C::kMl), plan);
+    ptx::fence_proxy_async_smem();                 // the plan's scratch becomes the V ring
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *slot;
+    Walker walk(p, *plan);
+    Item it;
+
+    if (warp >= kSoftmaxWarps) {
+    // ==================================================================== producer warpgroup
+    ptx::setmaxnreg_dec<kProducerRegs>();
+    if (warp == 8 || warp == 10) {
+        // ================================================================ producers: Q and K / V
+        const bool is_k = warp == 8;
+        const int NS = is_k ? C::kNK : C::kNV;
+        uint64_t* full = is_k ? k_full : v_full;
+        uint64_t* empty = is_k ? k_empty : v_empty;
+        const CUtensorMap* map = is_k ? &tmK : &tmV;
+        uint8_t* ring = smem + (is_k ? C::kK : C::kV);
+        const int nbox = 128 / p.box;
+        const int my_box = lane % nbox, my_half = p.split ? lane / nbox : 0;
+        const bool loads = lane < nbox * (p.split ? DH : 1);
+        uint32_t count = 0, qcount = 0;
+        bool ok = true;
+        if (lane == 0) ptx::prefetch_tensormap(map);
+        while (ok && walk.next(it)) {
+            if (is_k) {
+                // the piece's Q half tiles into the next half slots
+                for (int x = 0; x < (it.single ? 1 : 2) && ok; ++x, ++qcount) {
+                    const int sl = qcount & 1;
+                    if (lane == 0) {
+                        ok = qcount < 2 || ptx::mbar_wait(&q_empty[sl], ((qcount >> 1) & 1u) ^ 1u);
+                        if (ok) {
+                            ptx::mbar_arrive_expect_tx(&q_full[sl], (uint32_t)(p.TH * p.G * D * 2));
+                            for (int dh = 0; dh < DH; ++dh)
+                                ptx::tma_load_5d(smem + C::kQ + sl * C::kTile + dh * 16384, &tmQ, &q_full[sl], 0, 0,
+                                                 it.row0 + x * p.TH, dh, it.hk);
+                        }
+                    }
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                }
+            }
+            // this lane's page of the piece's key tiles, read one tile ahead;
+            // pages without a key that the tile sees are neither looked up nor read
+            const int32_t* row = p.table + (int64_t)it.b * p.table_stride;
+            auto page_of = [&](int t) -> int {
+                const int key = it.key0 + t * 128 + my_box * p.box;
+                if (!loads || t >= it.n || key >= it.j_hi || key + p.box <= it.j_lo) return -1;
+                return __ldg(row + key / p.page_size);
+            };
+            int nxt = page_of(0);
+            for (int t = 0; t < it.n && ok; ++t, ++count) {
+                int page = nxt;
+                nxt = page_of(t + 1);
+                const int key = it.key0 + t * 128 + my_box * p.box;
+                if (loads && key < it.j_hi && key + p.box > it.j_lo && (page < 0 || page >= p.num_pages)) {
+                    record_status(p.status, KESSIE_DEV_BAD_PAGE_ID);
+                    page = -1;
+                }
+                const int st = count % NS;
+                if (lane == 0) {
+                    ok = count < (uint32_t)NS || ptx::mbar_wait(&empty[st], ((count / NS) & 1u) ^ 1u);
+                    if (ok) ptx::mbar_arrive_expect_tx(&full[st], (uint32_t)C::kTile);
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (ok && loads) {
+                    const int tok = key % p.page_size;
+                    const int c4 = page < 0 ? p.oob_page : page * p.page_mul + it.hk * p.head_in_page;
+                    uint8_t* dst = ring + st * C::kTile;
+                    if (p.split) ptx::tma_load_5d(dst + my_half * 16384 + my_box * p.box * 128, map, &full[st], 0, tok, my_half, it.hk, c4);
+                    else ptx::tma_load_5d(dst + my_box * p.box * D * 2, map, &full[st], 0, 0, it.hk * p.head_in_row, tok >> 3, c4);
+                }
+                __syncwarp();
+            }
+        }
+        // every issued load has landed before the CTA can exit
+        if (lane == 0) {
+            if (!ok) record_status(p.status, KESSIE_DEV_WAIT_TIMEOUT);
+            for (uint32_t c = count > (uint32_t)NS ? count - NS : 0; c < count; ++c)
+                if (!ptx::mbar_wait(&full[c % NS], (c / NS) & 1u)) break;
+            for (uint32_t c = qcount > 2 ? qcount - 2 : 0; c < qcount; ++c)
+                if (!ptx::mbar_wait(&q_full[c & 1], (c >> 1) & 1u)) break;
+        }
+    } else if (warp == 9) {
+        // ================================================================ MMA issuer
+        const uint32_t idS = ptx::umma_idesc_f16(BF16, false, 128);
+        const uint32_t idPV = ptx::umma_idesc_f16(BF16, true, D);
+        // 8-row groups of a K/V tile: 1024 * DH apart with the halves interleaved, or 1024 in split half tiles
+        const uint32_t grp = p.split ? 1024u : 1024u * DH, half_off = p.split ? 16384u : 1024u;
+        uint32_t kc = 0, vc = 0, qc = 0, pc[2] = {0, 0}, items = 0;      // running stage / phase counters
+        bool ok = true;
+        while (ok && walk.next(it)) {
+            const int E = it.single ? it.n : 2 * it.n;
+            const uint32_t q_slot[2] = {qc & 1u, it.single ? (qc & 1u) : ((qc + 1) & 1u)};
+            auto key_tile = [&](int e) { return it.single ? e : e >> 1; };
+            auto issue_s = [&](int e) {
+                const int x = e & 1, t = key_tile(e);
+                const uint32_t st = (kc + t) % C::kNK;
+                if (it.single || x == 0) ok = ok && wait_all(&k_full[st], ((kc + t) / C::kNK) & 1u);
+                if (e < (it.single ? 1 : 2)) ok = ok && wait_all(&q_full[q_slot[x]], ((qc + x) >> 1) & 1u);
+                if (!ok) return;
+                ptx::tc_fence_after();
+                const uint32_t kb = ptx::smem_u32(smem + C::kK + st * C::kTile);
+                const uint32_t qb = ptx::smem_u32(smem + C::kQ + q_slot[x] * C::kTile);
+                if (lane == 0) {
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        ptx::umma_ss(tmem + x * 128, ptx::smem_desc_sw128(qb + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
+                                     ptx::smem_desc_sw128(kb + (kk >> 2) * half_off + (kk & 3) * 32, 16, grp), idS,
+                                     kk > 0 ? 1u : 0u);
+                    ptx::umma_commit(&s_full[x]);
+                    if (it.single || x == 1) ptx::umma_commit(&k_empty[st]);
+                    // the last scores of a half free its Q slot
+                    if (it.single ? e == E - 1 : e >= E - 2) ptx::umma_commit(&q_empty[q_slot[x]]);
+                }
+                __syncwarp();
+            };
+            issue_s(0);
+            if (ok && E > 1) issue_s(1);
+            for (int e = 0; e < E && ok; ++e) {
+                const int x = e & 1, t = key_tile(e);
+                const uint32_t st = (vc + t) % C::kNV;
+                if (it.single || x == 0) {
+                    ok = wait_all(&v_full[st], ((vc + t) / C::kNV) & 1u);
+                    const int key = it.key0 + t * 128;
+                    if (ok && (key + 128 > it.kv || key < it.j_lo)) {
+                        // rows of keys that no row of the tile sees (slots behind the last key, keys before
+                        // the window) may hold anything: zero them, so that 0 * NaN cannot reach O
+                        const int lo = max(0, it.j_lo - key), hi = min(128, max(0, it.kv - key));
+                        uint8_t* vt = smem + C::kV + st * C::kTile;
+                        for (int z = lane; z < 128 * DH * 8; z += 32) {
+                            const int r = z / (DH * 8), dh = (z >> 3) % DH, ch = z & 7;
+                            if (r >= lo && r < hi) continue;
+                            const uint32_t off = p.split ? dh * 16384 + r * 128 : (r >> 3) * 1024 * DH + dh * 1024 + (r & 7) * 128;
+                            *reinterpret_cast<uint4*>(vt + off + ch * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        ptx::fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                }
+                ok = ok && wait_all(&p_full[x], pc[x] & 1u);
+                ++pc[x];
+                if (ok && e == 0 && items > 0) ok = wait_all(o_free, (items - 1) & 1u);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                const uint32_t vb = ptx::smem_u32(smem + C::kV + st * C::kTile);
+                if (lane == 0) {
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk)
+                        ptx::umma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8,
+                                     ptx::smem_desc_sw128(vb + kk * 2 * grp, half_off, grp), idPV,
+                                     (e > 1 || kk > 0) ? 1u : 0u);
+                    if (it.single || x == 1) ptx::umma_commit(&v_empty[st]);
+                    if (e >= E - 2) ptx::umma_commit(&o_full[x]);
+                    if (E == 1) ptx::umma_commit(&o_full[1]);
+                }
+                __syncwarp();
+                if (e + 2 < E) issue_s(e + 2);
+            }
+            kc += it.n;
+            vc += it.n;
+            qc += it.single ? 1 : 2;
+            ++items;
+        }
+        if (!ok) record_status(p.status, KESSIE_DEV_WAIT_TIMEOUT);
+    } else if (FOG != kNoFog) {
+        // ================================================================ fog weights (warp 11)
+        uint32_t count = 0;
+        bool ok = true;
+        while (ok && walk.next(it)) {
+            const int edge = fog_edge<FOG>(p, it.b, it.kv);
+            const int n = fog_tiles<FOG>(p, it, edge);
+            const float inv_den = 1.f / (float)max(edge - 1, 1);
+            for (int t = 0; t < n && ok; ++t, ++count) {
+                const int st = count % kWStages;
+                if (count >= (uint32_t)kWStages) ok = wait_all(&w_empty[st], ((count / kWStages) & 1u) ^ 1u);
+                if (!ok) break;
+                float4 w4;
+                float* w = &w4.x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = it.key0 + t * 128 + lane * 4 + e;
+                    if (FOG == kValueFog)       // (key / (cs - 1))^alpha as 2^(alpha log2 ..), kessie_hip_kernels.py:411-412
+                        w[e] = key >= edge ? 1.f : ptx::ex2(p.fog_alpha * ptx::lg2((float)key * inv_den));
+                    else
+                        w[e] = key < it.kv ? fog_bias_at(p.bias, edge, key) * kLog2e : 0.f;
+                }
+                reinterpret_cast<float4*>(smem + C::kW)[st * 32 + lane] = w4;
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&w_full[st]);
+            }
+        }
+        if (!ok) record_status(p.status, KESSIE_DEV_WAIT_TIMEOUT);
+    }
+    } else {
+        // ================================================================ softmax warpgroups
+        ptx::setmaxnreg_inc<kSoftmaxRegs>();
+        const int x = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane;
+        const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+        const uint32_t sreg = tmem + lane_off + (uint32_t)(x * 128);
+        const uint32_t oreg = tmem + lane_off + 256;
+        const float* wring = reinterpret_cast<const float*>(smem + C::kW);
+        float2* mlbuf = reinterpret_cast<float2*>(smem + C::kMl);
+        uint32_t sc = 0, wc = 0, items = 0, singles = 0;
+        bool ok = true;
+        PieceDesc desc{0, 0, 0, 0, 0, 0, 0, 0};
+        while (ok && walk.next(it)) {
+            if (items == 0 && !it.first)
+                desc = PieceDesc{1, it.last ? 1 : 0, it.b, it.hk, it.tok0, it.ntok, it.row0, 0};
+            const int nev = it.single ? (it.n + 1 - x) >> 1 : it.n;
+            const int edge = fog_edge<FOG>(p, it.b, it.kv);
+            const int nw = fog_tiles<FOG>(p, it, edge);
+            // this thread's row: token and head of the group
+            const int base_tok = it.single ? 0 : x * p.TH;
+            const int tok = base_tok + r / p.G, gh = r % p.G;
+            const bool valid = r < p.TH * p.G && tok < it.ntok;
+            const bool any = __any_sync(0xffffffffu, valid);
+            const int pos = it.q0 + tok;
+            const bool limited = p.causal || p.window > 0;
+            int hi_r = limited ? min(it.kv, pos + 1) : it.kv;
+            int lo_r = p.window > 0 ? pos - p.window + 1 : 0;
+            if (!valid) hi_r = lo_r = 0;
+            // positions of the warp's rows, for the tiles that need no mask
+            const int w_lo = it.q0 + base_tok + (q4 * 32) / p.G;
+            const int w_hi = it.q0 + min(it.ntok - 1, base_tok + min(q4 * 32 + 31, p.TH * p.G - 1) / p.G);
+            float m_used = -INFINITY, l = 0.f;
+            for (int ev = 0; ev < nev; ++ev, ++sc) {
+                const int t = it.single ? 2 * ev + x : ev;
+                const int key0 = it.key0 + t * 128;
+                const bool weighted = FOG != kNoFog && t < nw;
+                const uint32_t wi = (wc + t) % kWStages;
+                if (weighted && !wait_all(&w_full[wi], ((wc + t) / kWStages) & 1u)) { ok = false; break; }
+                if (!wait_all(&s_full[x], sc & 1u)) { ok = false; break; }
+                if (any) {
+                    ptx::tc_fence_after();
+                    const float* wts = wring + wi * 128;
+                    uint32_t sv[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) ptx::tmem_ld32(sreg + c * 32, sv[c]);
+                    ptx::tmem_ld_wait();
+                    if (FOG == kScoreFog) {
+                        // to log2 units with the bias; the exponent below then has scale 1
+                        const uint64_t sc2 = ptx::f2_pack(p.scale_log2, p.scale_log2);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                uint64_t b2 = 0ull;
+                                if (weighted) b2 = *reinterpret_cast<const uint64_t*>(wts + c * 32 + 2 * i);
+                                float s0, s1;
+                                ptx::f2_unpack(ptx::ffma2(ptx::f2_pack(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1])), sc2, b2), s0, s1);
+                                sv[c][2 * i] = __float_as_uint(s0);
+                                sv[c][2 * i + 1] = __float_as_uint(s1);
+                            }
+                    }
+                    const float scale = FOG == kScoreFog ? 1.f : p.scale_log2;
+                    const bool interior = key0 + 128 <= it.kv && (!limited || key0 + 127 <= w_lo) &&
+                                          (p.window <= 0 || key0 >= w_hi - p.window + 1);
+                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    if (interior) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2)
+                                mx4[(i >> 1) & 3] = ptx::max3(mx4[(i >> 1) & 3], __uint_as_float(sv[c][i]), __uint_as_float(sv[c][i + 1]));
+                    } else {
+                        const int lo = lo_r - key0, hi = hi_r - key0;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const float s = (c * 32 + i >= lo && c * 32 + i < hi) ? __uint_as_float(sv[c][i]) : -INFINITY;
+                                sv[c][i] = __float_as_uint(s);
+                                mx4[i & 3] = fmaxf(mx4[i & 3], s);
+                            }
+                    }
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                    const float m_tile = mx == -INFINITY ? -INFINITY : mx * scale;
+                    const float m_new = fmaxf(m_used, m_tile);
+                    const bool need = m_new != -INFINITY && (m_used == -INFINITY || m_new > m_used + kRescaleThreshold);
+                    float factor = 1.f;
+                    if (need) {
+                        factor = m_used == -INFINITY ? 0.f : ptx::ex2(m_used - m_new);
+                        l *= factor;
+                        m_used = m_new;
+                    }
+                    const float nb = m_used == -INFINITY ? 0.f : -m_used;
+                    __syncwarp();                  // tcgen05.st is warp-collective
+                    if (FOG == kValueFog && weighted) l += softmax_p<BF16, true>(sv, sreg, scale, nb, wts);
+                    else l += softmax_p<BF16, false>(sv, sreg, scale, nb, wts);
+                    // O moves with the reference (rare): its last product is complete, the next waits for p_full
+                    if (__any_sync(0xffffffffu, need && factor != 0.f && ev > 0)) {
+                        const float f = need && factor != 0.f ? factor : 1.f;
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t ov[32];
+                            ptx::tmem_ld32(oreg + x * 128 + c * 32, ov);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
+                            ptx::tmem_st32(oreg + x * 128 + c * 32, ov);
+                        }
+                        ptx::tmem_st_wait();
+                    }
+                    ptx::tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive(&p_full[x]);
+                    if (weighted) mbar_arrive_n(&w_empty[wi], it.single ? 2 : 1);
+                }
+            }
+            if (!ok) break;
+            wc += nw;
+            // ---- end of the piece: O, m, l of this warp's rows
+            if (!wait_all(&o_full[x], items & 1u)) { ok = false; break; }
+            const bool mine = !it.single || x == 0;        // A writes a single tile for both chains
+            float f0 = 1.f, f1 = 0.f;
+            bool two = false;
+            if (it.single) {
+                if (x == 1) {
+                    mlbuf[r] = make_float2(m_used, l);
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(ml_full);
+                } else {
+                    if (!wait_all(&o_full[1], items & 1u) || !wait_all(ml_full, singles & 1u)) { ok = false; break; }
+                    const float2 o = mlbuf[r];
+                    const float m = fmaxf(m_used, o.x);
+                    f0 = m_used == -INFINITY ? 0.f : ptx::ex2(m_used - m);
+                    f1 = o.x == -INFINITY ? 0.f : ptx::ex2(o.x - m);
+                    l = l * f0 + o.y * f1;
+                    m_used = m;
+                    two = it.n > 1;
+                }
+                ++singles;
+            }
+            if (mine && any) {
+                ptx::tc_fence_after();
+                const bool whole = it.first && it.last;
+                const float inv = l > 0.f ? 1.f / l : 0.f;
+                uint16_t* orow = static_cast<uint16_t*>(p.o) + (int64_t)(it.row0 + tok) * p.o_st + (int64_t)(it.hk * p.G + gh) * p.o_sh;
+                char* part = p.ws + (size_t)gridDim.x * sizeof(PieceDesc) + (size_t)(2 * blockIdx.x + (it.first ? 1 : 0)) * C::kSlotBytes;
+                const int prow = it.single ? r : x * 128 + r;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t ov[32];
+                    ptx::tmem_ld32(oreg + x * 128 + c * 32, ov);
+                    ptx::tmem_ld_wait();
+                    if (it.single) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f0);
+                        if (two) {
+                            uint32_t o2[32];
+                            ptx::tmem_ld32(oreg + 128 + c * 32, o2);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(fmaf(__uint_as_float(o2[i]), f1, __uint_as_float(ov[i])));
+                        }
+                    }
+                    if (valid && whole) {
+                        uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
+                            uint32_t pk[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                pk[i] = ptx::pack2<BF16>(__uint_as_float(ov[8 * v + 2 * i]) * inv, __uint_as_float(ov[8 * v + 2 * i + 1]) * inv);
+                            dst[v] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                        }
+                    } else if (valid) {
+                        uint4* dst = reinterpret_cast<uint4*>(part) + (size_t)(c * 8) * 256 + prow;
+#pragma unroll
+                        for (int v = 0; v < 8; ++v) dst[v * 256] = make_uint4(ov[4 * v], ov[4 * v + 1], ov[4 * v + 2], ov[4 * v + 3]);
+                    }
+                    __syncwarp();                  // tcgen05.ld is warp-collective
+                }
+                if (valid && !whole) reinterpret_cast<float2*>(part + (size_t)256 * D * 4)[prow] = make_float2(m_used, l);
+                ptx::tc_fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(o_free);
+            ++items;
+        }
+        if (!ok) record_status(p.status, KESSIE_DEV_WAIT_TIMEOUT);
+        if (threadIdx.x == 0) reinterpret_cast<PieceDesc*>(p.ws)[blockIdx.x] = desc;
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+// Joins the pieces of cut tiles: block (c, y) takes 32 rows of the tile that
+// range boundary c (between CTAs c - 1 and c) is the first to cut.  Its pieces
+// are CTA c - 1's second slot and the first slots of c, c + 1, ... to the one
+// that ends the tile, joined in that order.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) fog_chunks_merge_kernel(const ChunkParams p, int ctas) {
+    const PieceDesc* desc = reinterpret_cast<const PieceDesc*>(p.ws);
+    const int c = blockIdx.x + 1;
+    const PieceDesc d = desc[c];
+    if (!d.mid) return;
+    if (desc[c - 1].mid && !desc[c - 1].ends) return;           // an earlier boundary cut this tile
+    int n = 1;                                                   // pieces after the first
+    for (int e = d.ends; !e && c + n < ctas; ++n) e = desc[c + n].ends;
+    const int rows = d.ntok <= p.TH ? d.ntok * p.G : p.TH * p.G + 128;
+    const char* slots = p.ws + (size_t)ctas * sizeof(PieceDesc);
+    auto slot = [&](int i) { return slots + (size_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c + i - 1)) * Cfg<D>::kSlotBytes; };
+    const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;   // a warp: 32 rows, 8 columns at a time
+    const int row = blockIdx.y * 32 + lane;
+    const int half = row >> 7, r = row & 127;
+    const int tok = half * p.TH + r / p.G;
+    if (row >= rows || r >= p.TH * p.G || tok >= d.ntok) return;
+    float m = -INFINITY;
+    for (int i = 0; i <= n; ++i) m = fmaxf(m, reinterpret_cast<const float2*>(slot(i) + (size_t)256 * D * 4)[row].x);
+    uint16_t* o = static_cast<uint16_t*>(p.o) + (int64_t)(d.row0 + tok) * p.o_st + (int64_t)(d.hk * p.G + r % p.G) * p.o_sh;
+    for (int c8 = grp; c8 < D / 8; c8 += 8) {
+        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
+        for (int i = 0; i <= n; ++i) {
+            const char* s = slot(i);
+            const float2 ml = reinterpret_cast<const float2*>(s + (size_t)256 * D * 4)[row];
+            const float f = ml.x == -INFINITY ? 0.f : ptx::ex2(ml.x - m);
+            const float4 a = reinterpret_cast<const float4*>(s)[(2 * c8) * 256 + row];
+            const float4 b = reinterpret_cast<const float4*>(s)[(2 * c8 + 1) * 256 + row];
+            l += ml.y * f;
+            acc[0] += a.x * f; acc[1] += a.y * f; acc[2] += a.z * f; acc[3] += a.w * f;
+            acc[4] += b.x * f; acc[5] += b.y * f; acc[6] += b.z * f; acc[7] += b.w * f;
+        }
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        uint32_t pk[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pk[i] = ptx::pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+        *reinterpret_cast<uint4*>(o + c8 * 8) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+    }
+}
+
+// Tensor map of K (or V); fills the box geometry of `p`.  The 8-row groups of
+// a box need (8 tokens, D/64, token / 8) as separate dimensions, which leaves
+// two for head and page: the head joins the 64-wide columns when heads are
+// adjacent (head stride D), or the page when the page stride is a multiple of
+// the head stride.  Other layouts load the 64-wide halves separately.
+CUresult encode_kv(CUtensorMap* map, const void* base, bool bf16, int D, int64_t page_stride, int64_t token_stride,
+                   int64_t head_stride, ChunkParams& p) {
+    const cuuint64_t DH = D / 64;
+    int box = 128;
+    while (p.page_size % box) box >>= 1;
+    p.box = box;
+    p.split = 0;
+    const cuuint64_t tok = (cuuint64_t)token_stride * 2, page = (cuuint64_t)page_stride * 2, head = (cuuint64_t)head_stride * 2;
+    if (head_stride == D || p.Hkv == 1) {
+        p.page_mul = 1; p.head_in_page = 0; p.head_in_row = (int)DH; p.oob_page = p.num_pages;
+        const cuuint64_t dims[5] = {64, 8, DH * p.Hkv, (cuuint64_t)p.page_size / 8, (cuuint64_t)p.num_pages};
+        const cuuint64_t str[4] = {tok, 128, 8 * tok, page};
+        const cuuint32_t bx[5] = {64, 8, (cuuint32_t)DH, (cuuint32_t)box / 8, 1};
+        return encode_tiled_5d_sw128(map, base, bf16, dims, str, bx);
+    }
+    const int64_t ratio = head_stride > 0 && page_stride % head_stride == 0 ? page_stride / head_stride : 0;
+    const int64_t merged = ratio > 0 ? (p.num_pages - 1) * ratio + p.Hkv : 0;
+    if (ratio >= p.Hkv && merged < INT_MAX) {
+        p.page_mul = (int)ratio; p.head_in_page = 1; p.head_in_row = 0; p.oob_page = (int)merged;
+        const cuuint64_t dims[5] = {64, 8, DH, (cuuint64_t)p.page_size / 8, (cuuint64_t)merged};
+        const cuuint64_t str[4] = {tok, 128, 8 * tok, head};
+        const cuuint32_t bx[5] = {64, 8, (cuuint32_t)DH, (cuuint32_t)box / 8, 1};
+        return encode_tiled_5d_sw128(map, base, bf16, dims, str, bx);
+    }
+    p.page_mul = 1; p.head_in_page = 0; p.head_in_row = 0; p.oob_page = p.num_pages; p.split = 1;
+    const cuuint64_t dims[5] = {64, (cuuint64_t)p.page_size, DH, (cuuint64_t)p.Hkv, (cuuint64_t)p.num_pages};
+    const cuuint64_t str[4] = {tok, 128, head, page};
+    const cuuint32_t bx[5] = {64, (cuuint32_t)box, 1, 1, 1};
+    return encode_tiled_5d_sw128(map, base, bf16, dims, str, bx);
+}
+
+template <int D, bool BF16, int FOG>
+int launch_chunks(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ChunkParams& p, int grid, cudaStream_t st) {
+    auto kern = fog_chunks_kernel<D, BF16, FOG>;
+    // setmaxnreg.inc draws on the registers of the launch: valid only if the kernel was built with kLaunchRegs
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) return check_launch("paged_fog_chunks: attributes");
+    if (fa.numRegs < kLaunchRegs)
+        return set_error(KESSIE_ERR_UNSUPPORTED, "paged_fog_chunks: built with %d registers", fa.numRegs);
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kAlloc) != cudaSuccess)
+        return check_launch("paged_fog_chunks: set smem attribute");
+    kern<<<grid, kThreads, Cfg<D>::kAlloc, st>>>(q, k, v, p);
+    const int rc = check_launch("paged_fog_chunks");
+    if (rc || grid < 2) return rc;
+    fog_chunks_merge_kernel<D, BF16><<<dim3(grid - 1, 8), 256, 0, st>>>(p, grid);
+    return check_launch("paged_fog_chunks merge");
+}
+
+template <int D, bool BF16>
+int launch_fog(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ChunkParams& p, int grid, cudaStream_t st) {
+    if (p.bias.on) return launch_chunks<D, BF16, kScoreFog>(q, k, v, p, grid, st);
+    if (p.clear_start) return launch_chunks<D, BF16, kValueFog>(q, k, v, p, grid, st);
+    return launch_chunks<D, BF16, kNoFog>(q, k, v, p, grid, st);
 }
 
 }  // namespace
@@ -84,7 +892,8 @@ __global__ void __launch_bounds__(128) fog_chunks_simple_kernel(const ChunkParam
 using namespace kessie;
 
 extern "C" size_t kessie_paged_fog_chunks_workspace_size(int num_q_heads, int num_kv_heads, int head_dim) {
-    return num_q_heads > 0 && num_kv_heads > 0 && head_dim > 0 ? 256 : 0;
+    if (num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0) return 0;
+    return (size_t)sm_count() * (sizeof(PieceDesc) + 2 * ((size_t)256 * head_dim * 4 + 256 * 8));
 }
 
 extern "C" int kessie_paged_fog_chunks_v2(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
@@ -123,26 +932,39 @@ extern "C" int kessie_paged_fog_chunks_v2(const void* q, int64_t q_stride_t, int
     const size_t need = kessie_paged_fog_chunks_workspace_size(num_q_heads, num_kv_heads, head_dim);
     if (!workspace || workspace_bytes < need)
         return set_error(KESSIE_ERR_WORKSPACE, "paged_fog_chunks_v2: workspace %zu < %zu", workspace_bytes, need);
+    if (batch > kMaxBatch)
+        return set_error(KESSIE_ERR_UNSUPPORTED, "paged_fog_chunks_v2: %d sequences (at most %d)", batch, kMaxBatch);
+    if (reinterpret_cast<uintptr_t>(workspace) & 15)
+        return set_error(KESSIE_ERR_WORKSPACE, "paged_fog_chunks_v2: workspace must be 16-byte aligned");
     ChunkParams p{};
-    p.q = q; p.q_st = q_stride_t; p.q_sh = q_stride_h;
     p.o = out; p.o_st = o_stride_t; p.o_sh = o_stride_h;
-    p.k = k_cache; p.v = v_cache;
-    p.page_stride = page_stride; p.token_stride = token_stride; p.head_stride = head_stride;
     p.num_pages = num_pages; p.page_size = page_size;
     p.table = block_table; p.table_stride = block_table_stride;
     p.start = query_start_loc; p.seq = seq_lens;
-    p.clear_start = clear_start; p.fog_alpha = fog_alpha;
+    p.clear_start = fog_alpha > 0.f ? clear_start : nullptr; p.fog_alpha = fog_alpha;
     p.window = window_size > 0 ? window_size : 0; p.causal = is_causal ? 1 : 0;
-    p.scale = sm_scale;
-    p.B = batch; p.T = num_tokens; p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.G = num_q_heads / num_kv_heads;
+    p.scale_log2 = sm_scale * kLog2e;
+    p.B = batch; p.T = num_tokens; p.Hkv = num_kv_heads; p.G = num_q_heads / num_kv_heads; p.TH = 128 / p.G;
     p.max_seq = max_seq_len;
     const int brc = fog_bias_from_c(bias, &p.bias);
     if (brc) return brc;
+    if (p.bias.on && p.clear_start)
+        return set_error(KESSIE_ERR_ARG, "paged_fog_chunks_v2: fog on the values or on the scores, not both");
     p.status = device_status_ptr();
-    const dim3 grid((num_q_heads + 3) / 4, batch);
-    auto kern = dtype == KESSIE_DTYPE_BF16
-                    ? (head_dim == 128 ? fog_chunks_simple_kernel<__nv_bfloat16, 128> : fog_chunks_simple_kernel<__nv_bfloat16, 64>)
-                    : (head_dim == 128 ? fog_chunks_simple_kernel<__half, 128> : fog_chunks_simple_kernel<__half, 64>);
-    kern<<<grid, 128, 0, as_stream(stream)>>>(p);
-    return check_launch("paged_fog_chunks");
+    p.ws = static_cast<char*>(workspace);
+    const bool bf16 = dtype == KESSIE_DTYPE_BF16;
+    CUtensorMap mq, mk, mv;
+    // q rows as {64 dims, head in group, token, 64-dim half, KV head}
+    const cuuint64_t dims[5] = {64, (cuuint64_t)p.G, (cuuint64_t)p.T, (cuuint64_t)head_dim / 64, (cuuint64_t)p.Hkv};
+    const cuuint64_t str[4] = {(cuuint64_t)q_stride_h * 2, (cuuint64_t)q_stride_t * 2, 128, (cuuint64_t)p.G * q_stride_h * 2};
+    const cuuint32_t bx[5] = {64, (cuuint32_t)p.G, (cuuint32_t)p.TH, 1, 1};
+    const CUresult rq = encode_tiled_5d_sw128(&mq, q, bf16, dims, str, bx);
+    const CUresult rk = encode_kv(&mk, k_cache, bf16, head_dim, page_stride, token_stride, head_stride, p);
+    const CUresult rv = encode_kv(&mv, v_cache, bf16, head_dim, page_stride, token_stride, head_stride, p);
+    if (rq != CUDA_SUCCESS || rk != CUDA_SUCCESS || rv != CUDA_SUCCESS)
+        return set_error(KESSIE_ERR_ARG, "paged_fog_chunks_v2: TMA descriptor rejected (q %d, k %d, v %d)", (int)rq, (int)rk, (int)rv);
+    const int grid = sm_count();
+    cudaStream_t st = as_stream(stream);
+    if (head_dim == 128) return bf16 ? launch_fog<128, true>(mq, mk, mv, p, grid, st) : launch_fog<128, false>(mq, mk, mv, p, grid, st);
+    return bf16 ? launch_fog<64, true>(mq, mk, mv, p, grid, st) : launch_fog<64, false>(mq, mk, mv, p, grid, st);
 }
