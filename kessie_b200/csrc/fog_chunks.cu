@@ -22,18 +22,24 @@
 // to end, each weighted with what it costs (kCostPair / kCostSingle per key
 // tile, kCostTile per tile), and the persistent grid's CTA c streams the
 // equal range [c L, (c + 1) L): no wave quantisation, whatever the mix of
-// lengths.  Every CTA derives the plan itself from the length arrays.  A tile
-// cut by a range boundary leaves fp32 partials (O, m, l) of each piece in the
+// lengths.  Cutting puts the CTAs at different keys of a head at any time, so
+// each would fetch its K/V for itself: when several tiles share a long context
+// (kWholeCost), the CTAs first take whole tiles in waves -- neighbours run
+// through the same keys together, from L2 -- and cut only what is left
+// (1,024-token chunk: see kWholeCost).  Every CTA derives the plan itself from
+// the length arrays.  A tile cut by a range boundary leaves fp32 partials (O, m, l) of each piece in the
 // workspace, at most two a CTA, and fog_chunks_merge_kernel joins them in
 // order, so results do not depend on timing.
 //
 // CTA = 12 warps: 0-3 / 4-7 softmax of A / B (one row per thread: TMEM lane =
-// row), 8 Q and K producer, 9 MMA issuer (one thread) and TMEM owner, 10 V
-// producer, 11 fog weights.  TMEM columns: S_A [0,128) S_B [128,256) O_A
-// [256,..) O_B [384,..); P (16-bit pairs) overwrites the first 64 columns of
-// its S.  Per event e (alternating A, B): wait P(e), O += P V, then S(e + 2) =
-// Q K^T into the region P(e) left, so one chain's MMAs run under the other's
-// softmax.  Producers run ahead over tile ends.
+// row), 8 Q and K producer, 9 / 11 MMA issuers of A / B (one thread each; 9
+// owns the TMEM), 10 V producer and fog weights.  TMEM columns: S_A [0,128) S_B
+// [128,256) O_A [256,..) O_B [384,..); P (16-bit pairs) overwrites the first 64
+// columns of its S.  Per key tile a chain's issuer waits for P, issues O += P V
+// and S = Q K^T of its next key tile into the region that P leaves, so one
+// chain's MMAs run under the other's softmax.  One issuer for both chains was
+// slower (4,600 against 3,600 cycles a pair of key tiles): its barrier waits
+// left the tensor pipe idle.  Producers run ahead over tile ends.
 //
 // K/V come straight from the pages: one TMA box per page (up to 128 tokens)
 // lands as [token / 8][D / 64][8][64] with 128-byte swizzle, whose 8-row groups
@@ -49,6 +55,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <atomic>
+
 namespace kessie {
 namespace {
 
@@ -59,11 +67,15 @@ constexpr int kWStages = 4;                  // key tiles of fog weights in flig
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;    // log2 units the running max may lag behind
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kProducerRegs = 64;
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kProducerRegs = 88;
 static_assert(256 * kSoftmaxRegs + 128 * kProducerRegs <= kThreads * kLaunchRegs, "register split exceeds the pool");
 
 // Plan weights of a 128-key tile (pair / single) and of starting and ending a tile.
 constexpr int kCostPair = 3, kCostSingle = 2, kCostTile = 4;
+
+// Whole tiles in waves first when the mean tile costs at least this (8k keys; at 2,048 tokens over 65k keys the pure
+// cut read 6.2 GB for 0.27 GB of K/V), at most kMaxWhole a CTA.
+constexpr int kWholeCost = 64 * kCostPair, kMaxWhole = 128;
 
 enum FogMode { kNoFog = 0, kValueFog = 1, kScoreFog = 2 };
 
@@ -98,17 +110,24 @@ template <int D> struct Cfg {
     static constexpr int kBar = kMl + 128 * 8;
     static constexpr int kNumBar = 4 + 2 * kNK + 2 * kNV + 2 * kWStages + 2 + 2 + 2 + 2;
     static constexpr int kPlan = kBar + kNumBar * 8;   // plan result and TMEM slot
-    static constexpr int kBytes = kPlan + 64;
+    static constexpr int kWalk = kPlan + 96;           // a Walker per warp
+    static constexpr int kWhole = kWalk + (kThreads / 32) * 128;   // whole tiles of this CTA
+    static constexpr int kBytes = kWhole + kMaxWhole * 12;
     static constexpr int kAlloc = kBytes + 1024;
-    static_assert(kNV * kTile >= kMaxBatch * 8, "the plan's prefix sums use the V ring");
+    static_assert(kNV * kTile >= kMaxBatch * 8 && kNK * kTile >= kMaxBatch * 4, "the plan's prefix sums use the rings");
     // partial slot in the workspace: O float4 [D / 4][256 rows], (m, l) float2 [256]
     static constexpr size_t kSlotBytes = (size_t)256 * D * 4 + 256 * 8;
 };
 
-// What the merge needs to know of CTA c's first piece.
-struct PieceDesc { int mid, ends, b, hk, tok0, ntok, row0, pad; };
+// What the merge needs to know of a CTA's range: no pieces, a first piece that starts its tile, or one that does not.
+enum PieceState { kNoPiece = 0, kStartsTile = 1, kMidTile = 2 };
+struct PieceDesc { int state, ends, b, hk, tok0, ntok, row0, pad; };
 
 struct Seq { int n, q0, kv, row0; };
+
+// This CTA's range [u0, u1) of the plan and the tile (sequence b, KV head hk, tile i, at pos) that u0 lies in.
+struct Plan { int64_t u0, u1, pos; int b, hk, i, any; Seq s; int whole; };
+struct WholeTile { int b, hk, i; };
 
 __device__ __forceinline__ Seq load_seq(const ChunkParams& p, int b, bool* bad = nullptr) {
     const int s0 = __ldg(p.start + b), s1 = __ldg(p.start + b + 1), len = __ldg(p.seq + b);
@@ -147,7 +166,7 @@ __device__ __forceinline__ int key_tile_at(const TileKeys& k, int64_t x) {
     return y <= 0 ? 0 : (int)min(y / w, (int64_t)(k.t_hi - k.t_lo));
 }
 
-struct Plan { int64_t u0, u1, pos; int b, hk, i, any; };
+
 
 // One piece of work: key tiles [k0, k1) of tile i of (b, hk).
 struct Item {
@@ -157,26 +176,48 @@ struct Item {
     bool single, first, last; // one half; starts / ends with its tile
 };
 
-// Walks the pieces of this CTA's range; every warp role walks them alike.
+// Walks the pieces of this CTA's range.  Every warp walks them for itself, in
+// shared memory: lane 0 steps, all lanes read the piece.
 struct Walker {
-    const ChunkParams& p;
     int64_t u0, u1, pos;
-    int b, hk, i;
+    const WholeTile* tiles;
+    int b, hk, i, whole;
     Seq s;
-    bool more;
-    __device__ Walker(const ChunkParams& p_, const Plan& pl) : p(p_), u0(pl.u0), u1(pl.u1), pos(pl.pos), b(pl.b),
-                                                              hk(pl.hk), i(pl.i), more(pl.any != 0) {
-        if (more) s = load_seq(p, b);
+    bool more, has;
+    Item it;
+    __device__ void begin(const Plan& pl, const WholeTile* list, int lane) {
+        if (lane == 0) {
+            tiles = list; whole = pl.whole;
+            u0 = pl.u0; u1 = pl.u1; pos = pl.pos; b = pl.b; hk = pl.hk; i = pl.i; s = pl.s; more = pl.any != 0;
+        }
+        __syncwarp();
     }
-    __device__ bool next(Item& it) {
+    __device__ bool next(const ChunkParams& p, int lane) {
+        __syncwarp();
+        if (lane == 0) has = step(p);
+        __syncwarp();
+        return has;
+    }
+    __device__ void piece(const ChunkParams& p, const Seq& q, const TileKeys& k, int b_, int hk_, int i_, int a, int e) {
+        it.b = b_; it.hk = hk_; it.tok0 = i_ * 2 * p.TH; it.ntok = k.ntok; it.row0 = q.row0 + it.tok0;
+        it.q0 = q.q0 + it.tok0; it.kv = q.kv; it.j_lo = k.j_lo; it.j_hi = k.j_hi;
+        it.key0 = (k.t_lo + a) << 7; it.n = e - a; it.single = k.single;
+        it.first = a == 0; it.last = e == k.t_hi - k.t_lo;
+    }
+    __device__ bool step(const ChunkParams& p) {
+        if (whole > 0) {
+            const WholeTile w = *tiles;
+            ++tiles;
+            --whole;
+            const Seq q = load_seq(p, w.b);
+            const TileKeys k = tile_keys(p, q, w.i);
+            piece(p, q, k, w.b, w.hk, w.i, 0, k.t_hi - k.t_lo);
+            return true;
+        }
         while (more) {
             const TileKeys k = tile_keys(p, s, i);
             const int cost = tile_cost(k);
-            const int a = key_tile_at(k, u0 - pos), e = key_tile_at(k, u1 - pos);
-            it.b = b; it.hk = hk; it.tok0 = i * 2 * p.TH; it.ntok = k.ntok; it.row0 = s.row0 + it.tok0;
-            it.q0 = s.q0 + it.tok0; it.kv = s.kv; it.j_lo = k.j_lo; it.j_hi = k.j_hi;
-            it.key0 = (k.t_lo + a) << 7; it.n = e - a; it.single = k.single;
-            it.first = a == 0; it.last = e == k.t_hi - k.t_lo;
+            piece(p, s, k, b, hk, i, key_tile_at(k, u0 - pos), key_tile_at(k, u1 - pos));
             // on to the next tile
             pos += cost;
             if (pos >= u1) more = false;
@@ -197,10 +238,53 @@ struct Walker {
     }
 };
 
-// This CTA's range of the plan (all threads; `pre` is shared scratch for B prefix sums).
-__device__ __forceinline__ void make_plan(const ChunkParams& p, int64_t* pre, int64_t* wsum, Plan* out) {
+// Inclusive sum over the block's threads of x; *total gets the whole sum.
+__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* wsum, int64_t* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+    }
+    if (lane == 31) wsum[warp] = x;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) x += wsum[w];
+        all += wsum[w];
+    }
+    __syncthreads();
+    *total = all;
+    return x;
+}
+// First index whose inclusive prefix (times mul) is above x.
+template <typename T>
+__device__ __forceinline__ int first_above(const T* pre, int n, int64_t mul, int64_t x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if ((int64_t)pre[mid] * mul > x) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+// The flat-th tile of the batch in (sequence, KV head, tile) order; cnt: prefix sums of the sequences' tiles.
+__device__ __forceinline__ WholeTile tile_of(const ChunkParams& p, const int* cnt, int64_t flat) {
+    WholeTile w;
+    w.b = first_above(cnt, p.B, p.Hkv, flat);
+    const int before = w.b ? cnt[w.b - 1] : 0, nt = cnt[w.b] - before;
+    const int rem = (int)(flat - (int64_t)before * p.Hkv);
+    w.hk = rem / nt;
+    w.i = rem - w.hk * nt;
+    return w;
+}
+
+// This CTA's share of the plan (all threads; pre and cnt: shared scratch for B prefix sums of cost and tiles).
+__device__ __forceinline__ void make_plan(const ChunkParams& p, int64_t* pre, int* cnt, int64_t* wsum, Plan* out,
+                                          WholeTile* list) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int64_t carry = 0;
+    const int64_t ctas = gridDim.x;
+    int64_t W = 0, tiles = 0;
     bool bad = false;
     const int TT = 2 * p.TH;
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
@@ -226,43 +310,70 @@ __device__ __forceinline__ void make_plan(const ChunkParams& p, int64_t* pre, in
             for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
             if (lane == src) c = x;
         }
-        c *= p.Hkv;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, c, d);
-            if (lane >= d) c += y;
+        // one scan for both sums: tiles (below 2^24: rows of q) above the cost (below 2^40)
+        int64_t all;
+        const int64_t both = block_scan(((int64_t)nt << 40) | (c * p.Hkv), wsum, &all);
+        const int64_t mask = (1ll << 40) - 1;
+        if (b < p.B) {
+            pre[b] = W + (both & mask);
+            cnt[b] = (int)(tiles + (both >> 40));
         }
-        if (lane == 31) wsum[warp] = c;
-        __syncthreads();
-        int64_t off = carry, all = 0;
-#pragma unroll
-        for (int w = 0; w < kThreads / 32; ++w) {
-            if (w < warp) off += wsum[w];
-            all += wsum[w];
-        }
-        if (b < p.B) pre[b] = off + c;
-        carry += all;
-        __syncthreads();
+        W += all & mask;
+        tiles += all >> 40;
     }
     if (bad && blockIdx.x == 0) record_status(p.status, KESSIE_DEV_BAD_ARG);
-    if (warp == 0) {
-        const int64_t W = carry;
-        // a range holds at least one key tile, so no piece between two others is empty
-        const int64_t L = max((W + gridDim.x - 1) / (int64_t)gridDim.x, (int64_t)(kCostTile + 2 * kCostPair));
-        const int64_t u0 = blockIdx.x * L;
-        Plan pl{u0, min(u0 + L, W), 0, 0, 0, 0, u0 < W ? 1 : 0};
-        if (pl.any) {
-            int lo = 0, hi = p.B - 1;                       // first b with pre[b] > u0
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (pre[mid] > u0) hi = mid; else lo = mid + 1;
+    __syncthreads();
+    // whole tiles first, where several share a long context
+    const int64_t n_tiles = tiles * p.Hkv;
+    int whole = 0;
+    if (W >= n_tiles * kWholeCost && n_tiles >= 2 * (int64_t)p.B * p.Hkv) whole = (int)min(n_tiles / ctas, (int64_t)kMaxWhole);
+    int64_t u_first = 0, u0, u1;
+    if (whole) {
+        // the cut part gives each CTA what its whole tiles leave of an equal share
+        int64_t share = 0, total;
+        if (tid < ctas) {
+            share = (W + ctas - 1) / ctas;
+            for (int k = 0; k < whole; ++k) {
+                const WholeTile w = tile_of(p, cnt, tid + k * ctas);
+                share -= tile_cost(tile_keys(p, load_seq(p, w.b), w.i));
             }
-            pl.b = lo;
-            const int64_t base = lo ? pre[lo - 1] : 0;
-            const int64_t per_head = (pre[lo] - base) / p.Hkv;
+            share = max(share, (int64_t)0);
+        }
+        if (tid < whole) list[tid] = tile_of(p, cnt, blockIdx.x + tid * ctas);
+        const int64_t upto = block_scan(share, wsum, &total);
+        if (tid == blockIdx.x) { wsum[16] = upto - share; wsum[17] = upto; }
+        __syncthreads();
+        u_first = W;
+        if (whole * ctas < n_tiles) {
+            const WholeTile w = tile_of(p, cnt, whole * ctas);
+            const Seq s = load_seq(p, w.b);
+            const int64_t base = w.b ? pre[w.b - 1] : 0;
+            u_first = base + w.hk * ((pre[w.b] - base) / p.Hkv);
+            int64_t x = 0;
+            for (int i = lane; i < w.i; i += 32) x += tile_cost(tile_keys(p, s, i));
+#pragma unroll
+            for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+            u_first += x;
+        }
+        const double f = total > 0 ? (double)(W - u_first) / (double)total : 0.0;
+        u0 = u_first + (int64_t)((double)wsum[16] * f);
+        u1 = blockIdx.x == ctas - 1 ? W : u_first + (int64_t)((double)wsum[17] * f);
+    } else {
+        // at least one key tile a range
+        const int64_t L = max((W + ctas - 1) / ctas, (int64_t)(2 * kCostPair));
+        u0 = min(blockIdx.x * L, W);
+        u1 = min(u0 + L, W);
+    }
+    if (warp == 0) {
+        Plan pl{u0, u1, 0, 0, 0, 0, u0 < u1 ? 1 : 0, Seq{0, 0, 0, 0}, whole};
+        if (pl.any) {
+            pl.b = first_above(pre, p.B, 1, u0);
+            const int64_t base = pl.b ? pre[pl.b - 1] : 0;
+            const int64_t per_head = (pre[pl.b] - base) / p.Hkv;
             pl.hk = (int)((u0 - base) / per_head);
             int64_t at = base + pl.hk * per_head;
-            const Seq s = load_seq(p, lo);
+            const Seq s = load_seq(p, pl.b);
+            pl.s = s;
             for (int i0 = 0;; i0 += 32) {
                 const int i = i0 + lane;
                 int64_t c = i * TT < s.n ? tile_cost(tile_keys(p, s, i)) : 0;
@@ -291,6 +402,28 @@ __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, int n) {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0], %1;\n\t}"
                  :: "r"(ptx::smem_u32(bar)), "r"(n) : "memory");
 }
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+// tcgen05.mma with the operand descriptors as two words each: stepping through
+// an operand only adds to the low word (the address field), so a step costs
+// the issuing thread one 32-bit add instead of rebuilding a 64-bit descriptor.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
+__device__ __forceinline__ uint32_t desc_hi(uint32_t sbo) { return (sbo >> 4) | 1u << 14 | 2u << 29; }
+template <bool ACCUM>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t alo, uint32_t ahi, uint32_t blo, uint32_t bhi, uint32_t idesc) {
+    asm volatile("{\n\t.reg .b64 a, b;\n\t.reg .pred p;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+                 "setp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}"
+                 :: "r"(d), "r"(alo), "r"(ahi), "r"(blo), "r"(bhi), "r"(idesc), "n"(ACCUM ? 1 : 0) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t blo, uint32_t bhi, uint32_t idesc, uint32_t accum) {
+    asm volatile("{\n\t.reg .b64 b;\n\t.reg .pred p;\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
+                 :: "r"(d), "r"(a), "r"(blo), "r"(bhi), "r"(idesc), "r"(accum) : "memory");
+}
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity));
 }
@@ -310,6 +443,31 @@ __device__ __forceinline__ int fog_edge(const ChunkParams& p, int b, int kv) {
     return 0;
 }
 
+// Score-fog bias of the four keys from `key` (a multiple of 4), times log2 e:
+// fog_bias_at without branches, so that the four run side by side.  The
+// product with the double reciprocal rounds to the same fp32 as the division:
+// a quotient of two 24-bit numbers is never within 2^-50 (relative) of a
+// midpoint of fp32.
+__device__ __forceinline__ float4 score_fog4(const FogBias& f, int fb, double inv_fb, int key, int kv) {
+    uint32_t bits = 0;
+    if (f.recall && key < f.recall_nbits) bits = __ldg(f.recall + (key >> 5)) >> (key & 31);
+    const float boost = fog_bias_round(f.boost, f.round_mode) * kLog2e;
+    float4 out;
+    float* w = &out.x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int j = key + e, m = f.round_mode;
+        const float pos = fog_bias_round((float)j, m);
+        const float t = fog_bias_round((float)((double)pos * inv_fb), m);
+        float d = fog_bias_round(1.0f - t, m);
+        d = fog_bias_round(d * d, m);
+        d = j < fb ? fog_bias_round(d * f.neg_alpha, m) * kLog2e : 0.f;
+        if (j < f.recall_nbits && ((bits >> e) & 1u)) d = boost;
+        w[e] = j < kv ? d : 0.f;
+    }
+    return out;
+}
+
 // p = 2^(s * scale + nb) of one row's 128 scores, packed to 16-bit pairs over
 // the first 64 columns of the row's S; FOG == kValueFog with `wts`: p * w is
 // packed.  Returns the row sum of the unweighted, unrounded p.
@@ -321,17 +479,18 @@ __device__ __forceinline__ float softmax_p(const uint32_t (&sv)[4][32], uint32_t
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         uint32_t pk[16];
+        ulonglong2 w = {0ull, 0ull};
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const uint64_t s2 = ptx::f2_pack(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1]));
             float e0, e1;
             ptx::f2_unpack(ptx::ffma2(s2, sc2, nb2), e0, e1);
             float p0 = ptx::ex2(e0), p1 = ptx::ex2(e1);
-            sum[i & 1] = ptx::fadd2(sum[i & 1], ptx::f2_pack(p0, p1));
+            const uint64_t p2 = ptx::f2_pack(p0, p1);
+            sum[i & 1] = ptx::fadd2(sum[i & 1], p2);
             if (WEIGHTED) {
-                const float2 w = *reinterpret_cast<const float2*>(wts + c * 32 + 2 * i);
-                p0 *= w.x;
-                p1 *= w.y;
+                if (!(i & 1)) w = *reinterpret_cast<const ulonglong2*>(wts + c * 32 + 2 * i);
+                ptx::f2_unpack(ptx::fmul2(p2, i & 1 ? w.y : w.x), p0, p1);
             }
             pk[i] = ptx::pack2<BF16>(p0, p1);
         }
@@ -368,16 +527,16 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
     uint64_t* o_free = o_full + 2;                 // every softmax warp is done with the piece's O
     uint64_t* ml_full = o_free + 1;                // B's (m, l) of a single tile
     Plan* plan = reinterpret_cast<Plan*>(smem + C::kPlan);
-    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::kPlan + 48);
+    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::kPlan + 80);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            ptx::mbar_init(&q_full[i], 1); ptx::mbar_init(&q_empty[i], 1);
+            ptx::mbar_init(&q_full[i], 1); ptx::mbar_init(&q_empty[i], 2);
             ptx::mbar_init(&s_full[i], 1); ptx::mbar_init(&p_full[i], 4); ptx::mbar_init(&o_full[i], 1);
         }
-        for (int i = 0; i < C::kNK; ++i) { ptx::mbar_init(&k_full[i], 1); ptx::mbar_init(&k_empty[i], 1); }
-        for (int i = 0; i < C::kNV; ++i) { ptx::mbar_init(&v_full[i], 1); ptx::mbar_init(&v_empty[i], 1); }
+        for (int i = 0; i < C::kNK; ++i) { ptx::mbar_init(&k_full[i], 1); ptx::mbar_init(&k_empty[i], 2); }
+        for (int i = 0; i < C::kNV; ++i) { ptx::mbar_init(&v_full[i], 1); ptx::mbar_init(&v_empty[i], 2); }
         for (int i = 0; i < kWStages; ++i) { ptx::mbar_init(&w_full[i], 1); ptx::mbar_init(&w_empty[i], kSoftmaxWarps); }
         ptx::mbar_init(o_free, kSoftmaxWarps);
         ptx::mbar_init(ml_full, 4);
@@ -387,14 +546,17 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
         ptx::tmem_alloc(slot, kTmemCols);
         ptx::tmem_relinquish();
     }
-    make_plan(p, reinterpret_cast<int64_t*>(smem + C::kV), reinterpret_cast<int64_t*>(smem + C::kMl), plan);
-    ptx::fence_proxy_async_smem();                 // the plan's scratch becomes the V ring
+    make_plan(p, reinterpret_cast<int64_t*>(smem + C::kV), reinterpret_cast<int*>(smem + C::kK),
+              reinterpret_cast<int64_t*>(smem + C::kMl), plan, reinterpret_cast<WholeTile*>(smem + C::kWhole));
+    ptx::fence_proxy_async_smem();                 // the plan's scratch becomes the K and V rings
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = *slot;
-    Walker walk(p, *plan);
-    Item it;
+    static_assert(sizeof(Walker) <= 128 && sizeof(Plan) <= 80, "plan and walker slots");
+    Walker& walk = *reinterpret_cast<Walker*>(smem + C::kWalk + warp * 128);
+    walk.begin(*plan, reinterpret_cast<const WholeTile*>(smem + C::kWhole), lane);
+    const Item& it = walk.it;
 
     if (warp >= kSoftmaxWarps) {
     // ==================================================================== producer warpgroup
@@ -410,10 +572,10 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
         const int nbox = 128 / p.box;
         const int my_box = lane % nbox, my_half = p.split ? lane / nbox : 0;
         const bool loads = lane < nbox * (p.split ? DH : 1);
-        uint32_t count = 0, qcount = 0;
+        uint32_t count = 0, qcount = 0, wcount = 0;
         bool ok = true;
         if (lane == 0) ptx::prefetch_tensormap(map);
-        while (ok && walk.next(it)) {
+        while (ok && walk.next(p, lane)) {
             if (is_k) {
                 // the piece's Q half tiles into the next half slots
                 for (int x = 0; x < (it.single ? 1 : 2) && ok; ++x, ++qcount) {
@@ -439,6 +601,32 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                 return __ldg(row + key / p.page_size);
             };
             int nxt = page_of(0);
+            // fog weights of key tile t, two tiles ahead of its V: that V's stage was free, so this slot is
+            const int edge = is_k ? 0 : fog_edge<FOG>(p, it.b, it.kv);
+            const int nw = is_k ? 0 : fog_tiles<FOG>(p, it, edge);
+            const float inv_den = 1.f / (float)max(edge - 1, 1);
+            const double inv_fb = FOG == kScoreFog ? 1.0 / (double)(float)max(edge, 1) : 0.0;
+            auto weights = [&](int t) {
+                if (FOG == kNoFog || t >= nw) return;
+                const uint32_t c = wcount++;
+                const int st = c % kWStages;
+                if (c >= (uint32_t)kWStages && !wait_all(&w_empty[st], ((c / kWStages) & 1u) ^ 1u)) { ok = false; return; }
+                float4 w4;
+                const int key = it.key0 + t * 128 + lane * 4;
+                if (FOG == kValueFog) {         // (key / (cs - 1))^alpha as 2^(alpha log2 ..), kessie_hip_kernels.py:411-412
+                    float* w = &w4.x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = key + e >= edge ? 1.f : ptx::ex2(p.fog_alpha * ptx::lg2((float)(key + e) * inv_den));
+                } else {
+                    w4 = score_fog4(p.bias, edge, inv_fb, key, it.kv);
+                }
+                reinterpret_cast<float4*>(smem + C::kW)[st * 32 + lane] = w4;
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&w_full[st]);
+            };
+            weights(0);
+            weights(1);
             for (int t = 0; t < it.n && ok; ++t, ++count) {
                 int page = nxt;
                 nxt = page_of(t + 1);
@@ -461,6 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                     else ptx::tma_load_5d(dst + my_box * p.box * D * 2, map, &full[st], 0, 0, it.hk * p.head_in_row, tok >> 3, c4);
                 }
                 __syncwarp();
+                weights(t + 2);
             }
         }
         // every issued load has landed before the CTA can exit
@@ -471,114 +660,79 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
             for (uint32_t c = qcount > 2 ? qcount - 2 : 0; c < qcount; ++c)
                 if (!ptx::mbar_wait(&q_full[c & 1], (c >> 1) & 1u)) break;
         }
-    } else if (warp == 9) {
-        // ================================================================ MMA issuer
+    } else if (elect_lane()) {
+        // ================================================================ MMA issuers: warp 9 chain A, warp 11 chain B
+        // A K or V stage is released by two arrivals: one of each chain (pair tiles), or two of the only one that
+        // used it (single tiles).  The piece's Q slots get one arrival of each chain, so that neither chain can pass
+        // a phase that the other still waits for.
+        const int x = warp == 9 ? 0 : 1;
         const uint32_t idS = ptx::umma_idesc_f16(BF16, false, 128);
         const uint32_t idPV = ptx::umma_idesc_f16(BF16, true, D);
         // 8-row groups of a K/V tile: 1024 * DH apart with the halves interleaved, or 1024 in split half tiles
         const uint32_t grp = p.split ? 1024u : 1024u * DH, half_off = p.split ? 16384u : 1024u;
-        uint32_t kc = 0, vc = 0, qc = 0, pc[2] = {0, 0}, items = 0;      // running stage / phase counters
+        const uint32_t q_base = ptx::smem_u32(smem + C::kQ), k_base = ptx::smem_u32(smem + C::kK), v_base = ptx::smem_u32(smem + C::kV);
+        const uint32_t q_hi = desc_hi(1024), kv_hi = desc_hi(grp);
+        const uint32_t tS = tmem + x * 128, tO = tmem + 256 + x * 128;
+        uint32_t tiles = 0, qc = 0, last_q = 0, pc = 0, items = 0;               // running stage / phase counters
         bool ok = true;
-        while (ok && walk.next(it)) {
-            const int E = it.single ? it.n : 2 * it.n;
-            const uint32_t q_slot[2] = {qc & 1u, it.single ? (qc & 1u) : ((qc + 1) & 1u)};
-            auto key_tile = [&](int e) { return it.single ? e : e >> 1; };
-            auto issue_s = [&](int e) {
-                const int x = e & 1, t = key_tile(e);
-                const uint32_t st = (kc + t) % C::kNK;
-                if (it.single || x == 0) ok = ok && wait_all(&k_full[st], ((kc + t) / C::kNK) & 1u);
-                if (e < (it.single ? 1 : 2)) ok = ok && wait_all(&q_full[q_slot[x]], ((qc + x) >> 1) & 1u);
+        Walker w = walk;                                             // this thread's own copy
+        while (ok && w.step(p)) {
+            const bool single = w.it.single;
+            const int n = w.it.n, nev = single ? (n + 1 - x) >> 1 : n;
+            const uint32_t slot_c = single ? qc : qc + x, q_slot = slot_c & 1u;
+            const uint32_t qlo = desc_lo(q_base + q_slot * C::kTile, 16);
+            auto issue_s = [&](int ev) {
+                const uint32_t t = tiles + (single ? 2 * ev + x : ev), st = t % C::kNK;
+                ok = ok && ptx::mbar_wait(&k_full[st], (t / C::kNK) & 1u);
                 if (!ok) return;
                 ptx::tc_fence_after();
-                const uint32_t kb = ptx::smem_u32(smem + C::kK + st * C::kTile);
-                const uint32_t qb = ptx::smem_u32(smem + C::kQ + q_slot[x] * C::kTile);
-                if (lane == 0) {
+                const uint32_t klo = desc_lo(k_base + st * C::kTile, 16);
+                mma_ss<false>(tS, qlo, q_hi, klo, kv_hi, idS);
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk)
-                        ptx::umma_ss(tmem + x * 128, ptx::smem_desc_sw128(qb + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
-                                     ptx::smem_desc_sw128(kb + (kk >> 2) * half_off + (kk & 3) * 32, 16, grp), idS,
-                                     kk > 0 ? 1u : 0u);
-                    ptx::umma_commit(&s_full[x]);
-                    if (it.single || x == 1) ptx::umma_commit(&k_empty[st]);
-                    // the last scores of a half free its Q slot
-                    if (it.single ? e == E - 1 : e >= E - 2) ptx::umma_commit(&q_empty[q_slot[x]]);
+                for (int kk = 1; kk < D / 16; ++kk)
+                    mma_ss<true>(tS, qlo + (kk >> 2) * 1024 + (kk & 3) * 2, q_hi,
+                                 klo + (kk >> 2) * (half_off >> 4) + (kk & 3) * 2, kv_hi, idS);
+                ptx::umma_commit(&s_full[x]);
+                ptx::umma_commit(&k_empty[st]);
+                if (single) ptx::umma_commit(&k_empty[st]);
+                if (ev == nev - 1) {                                 // the last scores: one arrival for each Q slot
+                    ptx::umma_commit(&q_empty[qc & 1u]);
+                    if (!single) ptx::umma_commit(&q_empty[(qc + 1) & 1u]);
                 }
-                __syncwarp();
             };
-            issue_s(0);
-            if (ok && E > 1) issue_s(1);
-            for (int e = 0; e < E && ok; ++e) {
-                const int x = e & 1, t = key_tile(e);
-                const uint32_t st = (vc + t) % C::kNV;
-                if (it.single || x == 0) {
-                    ok = wait_all(&v_full[st], ((vc + t) / C::kNV) & 1u);
-                    const int key = it.key0 + t * 128;
-                    if (ok && (key + 128 > it.kv || key < it.j_lo)) {
-                        // rows of keys that no row of the tile sees (slots behind the last key, keys before
-                        // the window) may hold anything: zero them, so that 0 * NaN cannot reach O
-                        const int lo = max(0, it.j_lo - key), hi = min(128, max(0, it.kv - key));
-                        uint8_t* vt = smem + C::kV + st * C::kTile;
-                        for (int z = lane; z < 128 * DH * 8; z += 32) {
-                            const int r = z / (DH * 8), dh = (z >> 3) % DH, ch = z & 7;
-                            if (r >= lo && r < hi) continue;
-                            const uint32_t off = p.split ? dh * 16384 + r * 128 : (r >> 3) * 1024 * DH + dh * 1024 + (r & 7) * 128;
-                            *reinterpret_cast<uint4*>(vt + off + ch * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        ptx::fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                }
-                ok = ok && wait_all(&p_full[x], pc[x] & 1u);
-                ++pc[x];
-                if (ok && e == 0 && items > 0) ok = wait_all(o_free, (items - 1) & 1u);
+            // Parity waits tell a phase only from its neighbours, and in a single tile a chain passes over the
+            // stages of the other: before this piece's first K, all scores of the last piece are done (its Q slots
+            // are free), before its first V, all products (o_free).
+            for (uint32_t c = qc - last_q; c != qc && ok; ++c) ok = ptx::mbar_wait(&q_empty[c & 1u], (c >> 1) & 1u);
+            last_q = single ? 1 : 2;
+            ok = ok && ptx::mbar_wait(&q_full[q_slot], (slot_c >> 1) & 1u);
+            if (ok && nev > 0) issue_s(0);
+            for (int ev = 0; ev < nev && ok; ++ev) {
+                const uint32_t t = tiles + (single ? 2 * ev + x : ev), st = t % C::kNV;
+                const uint32_t vlo = desc_lo(v_base + st * C::kTile, half_off);
+                // the first product overwrites O: the last piece's has been read
+                if (ev == 0 && items > 0) ok = ptx::mbar_wait(o_free, (items - 1) & 1u);
+                ok = ok && ptx::mbar_wait(&v_full[st], (t / C::kNV) & 1u);
+                ok = ok && ptx::mbar_wait(&p_full[x], pc & 1u);
+                ++pc;
                 if (!ok) break;
                 ptx::tc_fence_after();
-                const uint32_t vb = ptx::smem_u32(smem + C::kV + st * C::kTile);
-                if (lane == 0) {
+                mma_ts(tO, tS, vlo, kv_hi, idPV, ev > 0 ? 1u : 0u);
 #pragma unroll
-                    for (int kk = 0; kk < 8; ++kk)
-                        ptx::umma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8,
-                                     ptx::smem_desc_sw128(vb + kk * 2 * grp, half_off, grp), idPV,
-                                     (e > 1 || kk > 0) ? 1u : 0u);
-                    if (it.single || x == 1) ptx::umma_commit(&v_empty[st]);
-                    if (e >= E - 2) ptx::umma_commit(&o_full[x]);
-                    if (E == 1) ptx::umma_commit(&o_full[1]);
-                }
-                __syncwarp();
-                if (e + 2 < E) issue_s(e + 2);
+                for (int kk = 1; kk < 8; ++kk) mma_ts(tO, tS + kk * 8, vlo + kk * (grp >> 3), kv_hi, idPV, 1u);
+                if (ev == nev - 1) ptx::umma_commit(&o_full[x]);
+                ptx::umma_commit(&v_empty[st]);
+                if (single) ptx::umma_commit(&v_empty[st]);
+                if (ev + 1 < nev) issue_s(ev + 1);
             }
-            kc += it.n;
-            vc += it.n;
-            qc += it.single ? 1 : 2;
+            if (nev == 0 && ok) {                                    // a single tile's only key tile is chain A's
+                if (items > 0) ok = ptx::mbar_wait(o_free, (items - 1) & 1u);
+                ptx::mbar_arrive(&q_empty[q_slot]);
+                ptx::mbar_arrive(&o_full[x]);
+            }
+            tiles += n;
+            qc += single ? 1 : 2;
             ++items;
-        }
-        if (!ok) record_status(p.status, KESSIE_DEV_WAIT_TIMEOUT);
-    } else if (FOG != kNoFog) {
-        // ================================================================ fog weights (warp 11)
-        uint32_t count = 0;
-        bool ok = true;
-        while (ok && walk.next(it)) {
-            const int edge = fog_edge<FOG>(p, it.b, it.kv);
-            const int n = fog_tiles<FOG>(p, it, edge);
-            const float inv_den = 1.f / (float)max(edge - 1, 1);
-            for (int t = 0; t < n && ok; ++t, ++count) {
-                const int st = count % kWStages;
-                if (count >= (uint32_t)kWStages) ok = wait_all(&w_empty[st], ((count / kWStages) & 1u) ^ 1u);
-                if (!ok) break;
-                float4 w4;
-                float* w = &w4.x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = it.key0 + t * 128 + lane * 4 + e;
-                    if (FOG == kValueFog)       // (key / (cs - 1))^alpha as 2^(alpha log2 ..), kessie_hip_kernels.py:411-412
-                        w[e] = key >= edge ? 1.f : ptx::ex2(p.fog_alpha * ptx::lg2((float)key * inv_den));
-                    else
-                        w[e] = key < it.kv ? fog_bias_at(p.bias, edge, key) * kLog2e : 0.f;
-                }
-                reinterpret_cast<float4*>(smem + C::kW)[st * 32 + lane] = w4;
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&w_full[st]);
-            }
         }
         if (!ok) record_status(p.status, KESSIE_DEV_WAIT_TIMEOUT);
     }
@@ -591,12 +745,12 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
         const uint32_t oreg = tmem + lane_off + 256;
         const float* wring = reinterpret_cast<const float*>(smem + C::kW);
         float2* mlbuf = reinterpret_cast<float2*>(smem + C::kMl);
-        uint32_t sc = 0, wc = 0, items = 0, singles = 0;
+        uint32_t sc = 0, wc = 0, tiles = 0, items = 0, singles = 0;
         bool ok = true;
         PieceDesc desc{0, 0, 0, 0, 0, 0, 0, 0};
-        while (ok && walk.next(it)) {
-            if (items == 0 && !it.first)
-                desc = PieceDesc{1, it.last ? 1 : 0, it.b, it.hk, it.tok0, it.ntok, it.row0, 0};
+        while (ok && walk.next(p, lane)) {
+            if (!it.first) desc = PieceDesc{kMidTile, it.last ? 1 : 0, it.b, it.hk, it.tok0, it.ntok, it.row0, 0};
+            else if (!it.last && desc.state == kNoPiece) desc.state = kStartsTile;
             const int nev = it.single ? (it.n + 1 - x) >> 1 : it.n;
             const int edge = fog_edge<FOG>(p, it.b, it.kv);
             const int nw = fog_tiles<FOG>(p, it, edge);
@@ -613,14 +767,38 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
             // positions of the warp's rows, for the tiles that need no mask
             const int w_lo = it.q0 + base_tok + (q4 * 32) / p.G;
             const int w_hi = it.q0 + min(it.ntok - 1, base_tok + min(q4 * 32 + 31, p.TH * p.G - 1) / p.G);
+            // key tiles [t_in0, t_in1) need no mask for this warp's rows; from t_cut on (and before the window in the
+            // first) a key tile holds keys that no row of the tile sees
+            const bool single = it.single;
+            const int key_base = it.key0, kv = it.kv;
+            const int t_in1 = (min(kv, limited ? w_lo + 1 : kv) - key_base) >> 7;
+            const int t_in0 = p.window > 0 ? (w_hi - p.window + 1 - key_base + 127) >> 7 : 0;
+            const int t_cut = (kv - key_base) >> 7;
+            const bool cut_first = key_base < it.j_lo;
             float m_used = -INFINITY, l = 0.f;
             for (int ev = 0; ev < nev; ++ev, ++sc) {
-                const int t = it.single ? 2 * ev + x : ev;
-                const int key0 = it.key0 + t * 128;
+                const int t = single ? 2 * ev + x : ev;
                 const bool weighted = FOG != kNoFog && t < nw;
                 const uint32_t wi = (wc + t) % kWStages;
                 if (weighted && !wait_all(&w_full[wi], ((wc + t) / kWStages) & 1u)) { ok = false; break; }
                 if (!wait_all(&s_full[x], sc & 1u)) { ok = false; break; }
+                if (t >= t_cut || (cut_first && t == 0)) {
+                    // V rows of keys that no row of the tile sees (slots behind the last key, keys before the
+                    // window) may hold anything: zero them, so that 0 * NaN cannot reach O.  In a pair tile both
+                    // chains do (the same zeros).  o_free: see the issuers' first V.
+                    const uint32_t vt = tiles + t, st = vt % C::kNV;
+                    if (ev == 0 && items > 0 && !wait_all(o_free, (items - 1) & 1u)) { ok = false; break; }
+                    if (!wait_all(&v_full[st], (vt / C::kNV) & 1u)) { ok = false; break; }
+                    const int key0 = key_base + t * 128;
+                    const int lo = max(0, it.j_lo - key0), hi = min(128, max(0, kv - key0));
+                    uint8_t* vb = smem + C::kV + st * C::kTile;
+                    for (int z = r; z < 128 * DH * 8; z += 128) {
+                        const int vr = z / (DH * 8), dh = (z >> 3) % DH, ch = z & 7;
+                        const uint32_t off = p.split ? dh * 16384 + vr * 128 : (vr >> 3) * 1024 * DH + dh * 1024 + (vr & 7) * 128;
+                        if (vr < lo || vr >= hi) *reinterpret_cast<uint4*>(vb + off + ch * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    ptx::fence_proxy_async_smem();
+                }
                 if (any) {
                     ptx::tc_fence_after();
                     const float* wts = wring + wi * 128;
@@ -628,33 +806,34 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
 #pragma unroll
                     for (int c = 0; c < 4; ++c) ptx::tmem_ld32(sreg + c * 32, sv[c]);
                     ptx::tmem_ld_wait();
-                    if (FOG == kScoreFog) {
+                    float scale = p.scale_log2;
+                    if (FOG == kScoreFog && weighted) {
                         // to log2 units with the bias; the exponent below then has scale 1
-                        const uint64_t sc2 = ptx::f2_pack(p.scale_log2, p.scale_log2);
+                        const uint64_t sc2 = ptx::f2_pack(scale, scale);
+                        scale = 1.f;
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                uint64_t b2 = 0ull;
-                                if (weighted) b2 = *reinterpret_cast<const uint64_t*>(wts + c * 32 + 2 * i);
-                                float s0, s1;
-                                ptx::f2_unpack(ptx::ffma2(ptx::f2_pack(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1])), sc2, b2), s0, s1);
-                                sv[c][2 * i] = __float_as_uint(s0);
-                                sv[c][2 * i + 1] = __float_as_uint(s1);
+                            for (int i = 0; i < 32; i += 4) {
+                                const ulonglong2 b2 = *reinterpret_cast<const ulonglong2*>(wts + c * 32 + i);
+                                float s0, s1, s2, s3;
+                                ptx::f2_unpack(ptx::ffma2(ptx::f2_pack(__uint_as_float(sv[c][i]), __uint_as_float(sv[c][i + 1])), sc2, b2.x), s0, s1);
+                                ptx::f2_unpack(ptx::ffma2(ptx::f2_pack(__uint_as_float(sv[c][i + 2]), __uint_as_float(sv[c][i + 3])), sc2, b2.y), s2, s3);
+                                sv[c][i] = __float_as_uint(s0);
+                                sv[c][i + 1] = __float_as_uint(s1);
+                                sv[c][i + 2] = __float_as_uint(s2);
+                                sv[c][i + 3] = __float_as_uint(s3);
                             }
                     }
-                    const float scale = FOG == kScoreFog ? 1.f : p.scale_log2;
-                    const bool interior = key0 + 128 <= it.kv && (!limited || key0 + 127 <= w_lo) &&
-                                          (p.window <= 0 || key0 >= w_hi - p.window + 1);
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    if (interior) {
+                    if (t >= t_in0 && t < t_in1) {
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
 #pragma unroll
                             for (int i = 0; i < 32; i += 2)
                                 mx4[(i >> 1) & 3] = ptx::max3(mx4[(i >> 1) & 3], __uint_as_float(sv[c][i]), __uint_as_float(sv[c][i + 1]));
                     } else {
-                        const int lo = lo_r - key0, hi = hi_r - key0;
+                        const int lo = lo_r - key_base - t * 128, hi = hi_r - key_base - t * 128;
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -664,23 +843,22 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                                 mx4[i & 3] = fmaxf(mx4[i & 3], s);
                             }
                     }
-                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                    const float m_tile = mx == -INFINITY ? -INFINITY : mx * scale;
-                    const float m_new = fmaxf(m_used, m_tile);
-                    const bool need = m_new != -INFINITY && (m_used == -INFINITY || m_new > m_used + kRescaleThreshold);
-                    float factor = 1.f;
+                    const float m_tile = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
+                    // the reference moves when the maximum outgrows it by 2^8 (from -inf: at once)
+                    const bool need = m_tile > m_used + kRescaleThreshold;
+                    const float old = m_used;
                     if (need) {
-                        factor = m_used == -INFINITY ? 0.f : ptx::ex2(m_used - m_new);
+                        const float factor = ptx::ex2(m_used - m_tile);       // 0 from -inf
                         l *= factor;
-                        m_used = m_new;
+                        m_used = m_tile;
                     }
                     const float nb = m_used == -INFINITY ? 0.f : -m_used;
-                    __syncwarp();                  // tcgen05.st is warp-collective
+                    const bool moved = __any_sync(0xffffffffu, need && old != -INFINITY);
                     if (FOG == kValueFog && weighted) l += softmax_p<BF16, true>(sv, sreg, scale, nb, wts);
                     else l += softmax_p<BF16, false>(sv, sreg, scale, nb, wts);
                     // O moves with the reference (rare): its last product is complete, the next waits for p_full
-                    if (__any_sync(0xffffffffu, need && factor != 0.f && ev > 0)) {
-                        const float f = need && factor != 0.f ? factor : 1.f;
+                    if (moved) {
+                        const float f = need && old != -INFINITY ? ptx::ex2(old - m_used) : 1.f;
 #pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
                             uint32_t ov[32];
@@ -697,11 +875,12 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                 __syncwarp();
                 if (lane == 0) {
                     ptx::mbar_arrive(&p_full[x]);
-                    if (weighted) mbar_arrive_n(&w_empty[wi], it.single ? 2 : 1);
+                    if (weighted) mbar_arrive_n(&w_empty[wi], single ? 2 : 1);
                 }
             }
             if (!ok) break;
             wc += nw;
+            tiles += it.n;
             // ---- end of the piece: O, m, l of this warp's rows
             if (!wait_all(&o_full[x], items & 1u)) { ok = false; break; }
             const bool mine = !it.single || x == 0;        // A writes a single tile for both chains
@@ -774,6 +953,7 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
         if (!ok) record_status(p.status, KESSIE_DEV_WAIT_TIMEOUT);
         if (threadIdx.x == 0) reinterpret_cast<PieceDesc*>(p.ws)[blockIdx.x] = desc;
     }
+    __syncwarp();
     ptx::tc_fence_before();
     __syncthreads();
     if (warp == 9) {
@@ -782,22 +962,34 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
     }
 }
 
-// Joins the pieces of cut tiles: block (c, y) takes 32 rows of the tile that
-// range boundary c (between CTAs c - 1 and c) is the first to cut.  Its pieces
-// are CTA c - 1's second slot and the first slots of c, c + 1, ... to the one
-// that ends the tile, joined in that order.
+// Joins the pieces of cut tiles: block (c, y) takes 32 rows of the tile whose
+// second piece opens CTA c's range.  Its first piece is in the second slot of
+// the CTA before, the others in the first slots of c, c + 1, ... to the one
+// that ends the tile; they are joined in that order.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) fog_chunks_merge_kernel(const ChunkParams p, int ctas) {
     const PieceDesc* desc = reinterpret_cast<const PieceDesc*>(p.ws);
     const int c = blockIdx.x + 1;
     const PieceDesc d = desc[c];
-    if (!d.mid) return;
-    if (desc[c - 1].mid && !desc[c - 1].ends) return;           // an earlier boundary cut this tile
-    int n = 1;                                                   // pieces after the first
-    for (int e = d.ends; !e && c + n < ctas; ++n) e = desc[c + n].ends;
+    if (d.state != kMidTile) return;
+    int before = c - 1;                                          // the CTA with the piece before this one
+    while (before > 0 && desc[before].state == kNoPiece) --before;
+    if (desc[before].state == kMidTile && !desc[before].ends) return;      // an earlier boundary cut this tile
+    __shared__ int piece[kThreads];                              // the tile's pieces in order: slots
+    __shared__ int count;
+    if (threadIdx.x == 0) {
+        int n = 0;
+        piece[n++] = 2 * before + 1;
+        piece[n++] = 2 * c;
+        for (int e = d.ends, k = c + 1; !e && k < ctas; ++k)
+            if (desc[k].state == kMidTile) { piece[n++] = 2 * k; e = desc[k].ends; }
+        count = n;
+    }
+    __syncthreads();
+    const int n = count - 1;
     const int rows = d.ntok <= p.TH ? d.ntok * p.G : p.TH * p.G + 128;
     const char* slots = p.ws + (size_t)ctas * sizeof(PieceDesc);
-    auto slot = [&](int i) { return slots + (size_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c + i - 1)) * Cfg<D>::kSlotBytes; };
+    auto slot = [&](int i) { return slots + (size_t)piece[i] * Cfg<D>::kSlotBytes; };
     const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;   // a warp: 32 rows, 8 columns at a time
     const int row = blockIdx.y * 32 + lane;
     const int half = row >> 7, r = row & 127;
@@ -865,13 +1057,19 @@ CUresult encode_kv(CUtensorMap* map, const void* base, bool bf16, int D, int64_t
 template <int D, bool BF16, int FOG>
 int launch_chunks(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ChunkParams& p, int grid, cudaStream_t st) {
     auto kern = fog_chunks_kernel<D, BF16, FOG>;
-    // setmaxnreg.inc draws on the registers of the launch: valid only if the kernel was built with kLaunchRegs
-    cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) return check_launch("paged_fog_chunks: attributes");
-    if (fa.numRegs < kLaunchRegs)
-        return set_error(KESSIE_ERR_UNSUPPORTED, "paged_fog_chunks: built with %d registers", fa.numRegs);
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kAlloc) != cudaSuccess)
-        return check_launch("paged_fog_chunks: set smem attribute");
+    static std::atomic<uint64_t> ready{0};                    // devices on which the kernel is set up
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("paged_fog_chunks: device");
+    if (dev >= 64 || !((ready.load(std::memory_order_acquire) >> dev) & 1)) {
+        // setmaxnreg.inc draws on the registers of the launch: valid only if the kernel was built with kLaunchRegs
+        cudaFuncAttributes fa;
+        if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) return check_launch("paged_fog_chunks: attributes");
+        if (fa.numRegs < kLaunchRegs)
+            return set_error(KESSIE_ERR_UNSUPPORTED, "paged_fog_chunks: built with %d registers", fa.numRegs);
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kAlloc) != cudaSuccess)
+            return check_launch("paged_fog_chunks: set smem attribute");
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
     kern<<<grid, kThreads, Cfg<D>::kAlloc, st>>>(q, k, v, p);
     const int rc = check_launch("paged_fog_chunks");
     if (rc || grid < 2) return rc;
@@ -963,7 +1161,7 @@ extern "C" int kessie_paged_fog_chunks_v2(const void* q, int64_t q_stride_t, int
     const CUresult rv = encode_kv(&mv, v_cache, bf16, head_dim, page_stride, token_stride, head_stride, p);
     if (rq != CUDA_SUCCESS || rk != CUDA_SUCCESS || rv != CUDA_SUCCESS)
         return set_error(KESSIE_ERR_ARG, "paged_fog_chunks_v2: TMA descriptor rejected (q %d, k %d, v %d)", (int)rq, (int)rk, (int)rv);
-    const int grid = sm_count();
+    const int grid = sm_count() < kThreads ? sm_count() : kThreads;
     cudaStream_t st = as_stream(stream);
     if (head_dim == 128) return bf16 ? launch_fog<128, true>(mq, mk, mv, p, grid, st) : launch_fog<128, false>(mq, mk, mv, p, grid, st);
     return bf16 ? launch_fog<64, true>(mq, mk, mv, p, grid, st) : launch_fog<64, false>(mq, mk, mv, p, grid, st);
