@@ -35,9 +35,11 @@
 // row), 8 Q and K producer, 9 / 11 MMA issuers of A / B (one thread each; 9
 // owns the TMEM), 10 V producer and fog weights.  TMEM columns: S_A [0,128) S_B
 // [128,256) O_A [256,..) O_B [384,..); P (16-bit pairs) overwrites the first 64
-// columns of its S.  Per key tile a chain's issuer waits for P, issues O += P V
-// and S = Q K^T of its next key tile into the region that P leaves, so one
-// chain's MMAs run under the other's softmax.  One issuer for both chains was
+// columns of its S.  Per key tile a chain's issuer waits for P (in two halves, so
+// that the product starts under the second half's exponentials: 12.0 -> 11.7
+// Mcycles at 4,096 tokens over 131k keys), issues O += P V and S = Q K^T of its
+// next key tile into the region that P leaves, so one chain's MMAs run under the
+// other's softmax.  One issuer for both chains was
 // slower (4,600 against 3,600 cycles a pair of key tiles): its barrier waits
 // left the tensor pipe idle.  Producers run ahead over tile ends.
 //
@@ -108,7 +110,7 @@ template <int D> struct Cfg {
     static constexpr int kW = kV + kNV * kTile;        // fog weights
     static constexpr int kMl = kW + kWStages * 128 * 4;    // (m, l) of a single tile's B chain
     static constexpr int kBar = kMl + 128 * 8;
-    static constexpr int kNumBar = 4 + 2 * kNK + 2 * kNV + 2 * kWStages + 2 + 2 + 2 + 2;
+    static constexpr int kNumBar = 4 + 2 * kNK + 2 * kNV + 2 * kWStages + 2 + 2 + 2 + 2 + 2;
     static constexpr int kPlan = kBar + kNumBar * 8;   // plan result and TMEM slot
     static constexpr int kWalk = kPlan + 96;           // a Walker per warp
     static constexpr int kWhole = kWalk + (kThreads / 32) * 128;   // whole tiles of this CTA
@@ -161,9 +163,8 @@ __device__ __forceinline__ int tile_cost(const TileKeys& k) {
 }
 // Key tile of a tile's range at plan position x (relative to the tile's start).
 __device__ __forceinline__ int key_tile_at(const TileKeys& k, int64_t x) {
-    const int w = k.single ? kCostSingle : kCostPair;
-    const int64_t y = (x - kCostTile + w - 1);
-    return y <= 0 ? 0 : (int)min(y / w, (int64_t)(k.t_hi - k.t_lo));
+    const int y = (int)max((int64_t)0, min(x - kCostTile, (int64_t)INT_MAX - 8));
+    return min(k.single ? (y + kCostSingle - 1) / kCostSingle : (y + kCostPair - 1) / kCostPair, k.t_hi - k.t_lo);
 }
 
 
@@ -312,7 +313,7 @@ __device__ __forceinline__ void make_plan(const ChunkParams& p, int64_t* pre, in
         }
         // one scan for both sums: tiles (below 2^24: rows of q) above the cost (below 2^40)
         int64_t all;
-        const int64_t both = block_scan(((int64_t)nt << 40) | (c * p.Hkv), wsum, &all);
+        const int64_t both = block_scan(((int64_t)nt << 40) | c, wsum, &all);
         const int64_t mask = (1ll << 40) - 1;
         if (b < p.B) {
             pre[b] = W + (both & mask);
@@ -322,6 +323,7 @@ __device__ __forceinline__ void make_plan(const ChunkParams& p, int64_t* pre, in
         tiles += all >> 40;
     }
     if (bad && blockIdx.x == 0) record_status(p.status, KESSIE_DEV_BAD_ARG);
+    W *= p.Hkv;                                    // pre stays per head
     __syncthreads();
     // whole tiles first, where several share a long context
     const int64_t n_tiles = tiles * p.Hkv;
@@ -348,7 +350,7 @@ __device__ __forceinline__ void make_plan(const ChunkParams& p, int64_t* pre, in
             const WholeTile w = tile_of(p, cnt, whole * ctas);
             const Seq s = load_seq(p, w.b);
             const int64_t base = w.b ? pre[w.b - 1] : 0;
-            u_first = base + w.hk * ((pre[w.b] - base) / p.Hkv);
+            u_first = base * p.Hkv + w.hk * (pre[w.b] - base);
             int64_t x = 0;
             for (int i = lane; i < w.i; i += 32) x += tile_cost(tile_keys(p, s, i));
 #pragma unroll
@@ -367,10 +369,11 @@ __device__ __forceinline__ void make_plan(const ChunkParams& p, int64_t* pre, in
     if (warp == 0) {
         Plan pl{u0, u1, 0, 0, 0, 0, u0 < u1 ? 1 : 0, Seq{0, 0, 0, 0}, whole};
         if (pl.any) {
-            pl.b = first_above(pre, p.B, 1, u0);
-            const int64_t base = pl.b ? pre[pl.b - 1] : 0;
-            const int64_t per_head = (pre[pl.b] - base) / p.Hkv;
-            pl.hk = (int)((u0 - base) / per_head);
+            pl.b = first_above(pre, p.B, p.Hkv, u0);
+            const int64_t before = pl.b ? pre[pl.b - 1] : 0, per_head = pre[pl.b] - before;
+            const int64_t base = before * p.Hkv;
+            pl.hk = (u0 - base) >> 32 || per_head >> 32 ? (int)((u0 - base) / per_head)
+                                                        : (int)((uint32_t)(u0 - base) / (uint32_t)per_head);
             int64_t at = base + pl.hk * per_head;
             const Seq s = load_seq(p, pl.b);
             pl.s = s;
@@ -424,6 +427,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t blo, uin
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
                  :: "r"(d), "r"(a), "r"(blo), "r"(bhi), "r"(idesc), "r"(accum) : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity));
 }
@@ -468,18 +477,29 @@ __device__ __forceinline__ float4 score_fog4(const FogBias& f, int fb, double in
     return out;
 }
 
+// Four weights from shared memory, in program order: left to itself the
+// compiler gathers all 32 loads of a tile in front, and spills.
+__device__ __forceinline__ void lds_quad(ulonglong2& w, uint32_t saddr) {
+    asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(w.x), "=l"(w.y) : "r"(saddr));
+}
+
 // p = 2^(s * scale + nb) of one row's 128 scores, packed to 16-bit pairs over
 // the first 64 columns of the row's S; FOG == kValueFog with `wts`: p * w is
 // packed.  Returns the row sum of the unweighted, unrounded p.
 template <bool BF16, bool WEIGHTED>
 __device__ __forceinline__ float softmax_p(const uint32_t (&sv)[4][32], uint32_t sreg, float scale, float nb,
-                                           const float* wts) {
+                                           const float* wts, uint64_t* half_bar) {
     const uint64_t sc2 = ptx::f2_pack(scale, scale), nb2 = ptx::f2_pack(nb, nb);
     uint64_t sum[2] = {0ull, 0ull};
+    constexpr int kAhead = 1;
+    const uint32_t wa = WEIGHTED ? ptx::smem_u32(wts) : 0u;
+    ulonglong2 w[kAhead];
+    if (WEIGHTED)
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) lds_quad(w[k], wa + k * 16);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         uint32_t pk[16];
-        ulonglong2 w = {0ull, 0ull};
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const uint64_t s2 = ptx::f2_pack(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1]));
@@ -489,12 +509,19 @@ __device__ __forceinline__ float softmax_p(const uint32_t (&sv)[4][32], uint32_t
             const uint64_t p2 = ptx::f2_pack(p0, p1);
             sum[i & 1] = ptx::fadd2(sum[i & 1], p2);
             if (WEIGHTED) {
-                if (!(i & 1)) w = *reinterpret_cast<const ulonglong2*>(wts + c * 32 + 2 * i);
-                ptx::f2_unpack(ptx::fmul2(p2, i & 1 ? w.y : w.x), p0, p1);
+                const int quad = c * 8 + (i >> 1);
+                ptx::f2_unpack(ptx::fmul2(p2, i & 1 ? w[quad % kAhead].y : w[quad % kAhead].x), p0, p1);
+                if ((i & 1) && quad + kAhead < 32) lds_quad(w[quad % kAhead], wa + (quad + kAhead) * 16);
             }
             pk[i] = ptx::pack2<BF16>(p0, p1);
         }
         ptx::tmem_st16(sreg + c * 16, pk);
+        if (c == 1) {
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before();
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(half_bar);
+        }
     }
     ptx::tmem_st_wait();
     float a0, a1, b0, b1;
@@ -526,6 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
     uint64_t* o_full = p_full + 2;
     uint64_t* o_free = o_full + 2;                 // every softmax warp is done with the piece's O
     uint64_t* ml_full = o_free + 1;                // B's (m, l) of a single tile
+    uint64_t* ph_full = ml_full + 1;               // [2] first half of P
     Plan* plan = reinterpret_cast<Plan*>(smem + C::kPlan);
     uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::kPlan + 80);
 
@@ -533,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&q_full[i], 1); ptx::mbar_init(&q_empty[i], 2);
-            ptx::mbar_init(&s_full[i], 1); ptx::mbar_init(&p_full[i], 4); ptx::mbar_init(&o_full[i], 1);
+            ptx::mbar_init(&s_full[i], 1); ptx::mbar_init(&p_full[i], 4); ptx::mbar_init(&ph_full[i], 4); ptx::mbar_init(&o_full[i], 1);
         }
         for (int i = 0; i < C::kNK; ++i) { ptx::mbar_init(&k_full[i], 1); ptx::mbar_init(&k_empty[i], 2); }
         for (int i = 0; i < C::kNV; ++i) { ptx::mbar_init(&v_full[i], 1); ptx::mbar_init(&v_empty[i], 2); }
@@ -546,6 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
         ptx::tmem_alloc(slot, kTmemCols);
         ptx::tmem_relinquish();
     }
+    ptx::launch_dependents();                      // the merge waits for this grid's end by itself
     make_plan(p, reinterpret_cast<int64_t*>(smem + C::kV), reinterpret_cast<int*>(smem + C::kK),
               reinterpret_cast<int64_t*>(smem + C::kMl), plan, reinterpret_cast<WholeTile*>(smem + C::kWhole));
     ptx::fence_proxy_async_smem();                 // the plan's scratch becomes the K and V rings
@@ -713,13 +742,18 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                 // the first product overwrites O: the last piece's has been read
                 if (ev == 0 && items > 0) ok = ptx::mbar_wait(o_free, (items - 1) & 1u);
                 ok = ok && ptx::mbar_wait(&v_full[st], (t / C::kNV) & 1u);
-                ok = ok && ptx::mbar_wait(&p_full[x], pc & 1u);
-                ++pc;
+                ok = ok && ptx::mbar_wait(&ph_full[x], pc & 1u);
                 if (!ok) break;
                 ptx::tc_fence_after();
                 mma_ts(tO, tS, vlo, kv_hi, idPV, ev > 0 ? 1u : 0u);
 #pragma unroll
-                for (int kk = 1; kk < 8; ++kk) mma_ts(tO, tS + kk * 8, vlo + kk * (grp >> 3), kv_hi, idPV, 1u);
+                for (int kk = 1; kk < 4; ++kk) mma_ts(tO, tS + kk * 8, vlo + kk * (grp >> 3), kv_hi, idPV, 1u);
+                ok = ptx::mbar_wait(&p_full[x], pc & 1u);
+                ++pc;
+                if (!ok) break;
+                ptx::tc_fence_after();
+#pragma unroll
+                for (int kk = 4; kk < 8; ++kk) mma_ts(tO, tS + kk * 8, vlo + kk * (grp >> 3), kv_hi, idPV, 1u);
                 if (ev == nev - 1) ptx::umma_commit(&o_full[x]);
                 ptx::umma_commit(&v_empty[st]);
                 if (single) ptx::umma_commit(&v_empty[st]);
@@ -748,6 +782,9 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
         uint32_t sc = 0, wc = 0, tiles = 0, items = 0, singles = 0;
         bool ok = true;
         PieceDesc desc{0, 0, 0, 0, 0, 0, 0, 0};
+        const int r_tok = r / p.G, gh = r - r_tok * p.G;             // row: token of the half, head of the group
+        const int rows_half = p.TH * p.G;
+        const int w_tok0 = (q4 * 32) / p.G, w_tok1 = min(q4 * 32 + 31, rows_half - 1) / p.G;
         while (ok && walk.next(p, lane)) {
             if (!it.first) desc = PieceDesc{kMidTile, it.last ? 1 : 0, it.b, it.hk, it.tok0, it.ntok, it.row0, 0};
             else if (!it.last && desc.state == kNoPiece) desc.state = kStartsTile;
@@ -756,8 +793,8 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
             const int nw = fog_tiles<FOG>(p, it, edge);
             // this thread's row: token and head of the group
             const int base_tok = it.single ? 0 : x * p.TH;
-            const int tok = base_tok + r / p.G, gh = r % p.G;
-            const bool valid = r < p.TH * p.G && tok < it.ntok;
+            const int tok = base_tok + r_tok;
+            const bool valid = r < rows_half && tok < it.ntok;
             const bool any = __any_sync(0xffffffffu, valid);
             const int pos = it.q0 + tok;
             const bool limited = p.causal || p.window > 0;
@@ -765,8 +802,7 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
             int lo_r = p.window > 0 ? pos - p.window + 1 : 0;
             if (!valid) hi_r = lo_r = 0;
             // positions of the warp's rows, for the tiles that need no mask
-            const int w_lo = it.q0 + base_tok + (q4 * 32) / p.G;
-            const int w_hi = it.q0 + min(it.ntok - 1, base_tok + min(q4 * 32 + 31, p.TH * p.G - 1) / p.G);
+            const int w_lo = it.q0 + base_tok + w_tok0, w_hi = it.q0 + min(it.ntok - 1, base_tok + w_tok1);
             // key tiles [t_in0, t_in1) need no mask for this warp's rows; from t_cut on (and before the window in the
             // first) a key tile holds keys that no row of the tile sees
             const bool single = it.single;
@@ -790,12 +826,13 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                     if (ev == 0 && items > 0 && !wait_all(o_free, (items - 1) & 1u)) { ok = false; break; }
                     if (!wait_all(&v_full[st], (vt / C::kNV) & 1u)) { ok = false; break; }
                     const int key0 = key_base + t * 128;
-                    const int lo = max(0, it.j_lo - key0), hi = min(128, max(0, kv - key0));
+                    const int lo = min(128, max(0, it.j_lo - key0)), hi = min(128, max(lo, kv - key0));
                     uint8_t* vb = smem + C::kV + st * C::kTile;
-                    for (int z = r; z < 128 * DH * 8; z += 128) {
-                        const int vr = z / (DH * 8), dh = (z >> 3) % DH, ch = z & 7;
+                    const int n_zero = (lo + 128 - hi) * DH * 8;                  // rows [0, lo) and [hi, 128)
+                    for (int z = r; z < n_zero; z += 128) {
+                        const int zr = z / (DH * 8), vr = zr < lo ? zr : zr - lo + hi, dh = (z >> 3) % DH, ch = z & 7;
                         const uint32_t off = p.split ? dh * 16384 + vr * 128 : (vr >> 3) * 1024 * DH + dh * 1024 + (vr & 7) * 128;
-                        if (vr < lo || vr >= hi) *reinterpret_cast<uint4*>(vb + off + ch * 16) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(vb + off + ch * 16) = make_uint4(0, 0, 0, 0);
                     }
                     ptx::fence_proxy_async_smem();
                 }
@@ -811,11 +848,17 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                         // to log2 units with the bias; the exponent below then has scale 1
                         const uint64_t sc2 = ptx::f2_pack(scale, scale);
                         scale = 1.f;
+                        const uint32_t wa = ptx::smem_u32(wts);
+                        ulonglong2 ahead[2];
+                        lds_quad(ahead[0], wa);
+                        lds_quad(ahead[1], wa + 16);
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
 #pragma unroll
                             for (int i = 0; i < 32; i += 4) {
-                                const ulonglong2 b2 = *reinterpret_cast<const ulonglong2*>(wts + c * 32 + i);
+                                const int quad = c * 8 + (i >> 2);
+                                const ulonglong2 b2 = ahead[quad & 1];
+                                if (quad + 2 < 32) lds_quad(ahead[quad & 1], wa + (quad + 2) * 16);
                                 float s0, s1, s2, s3;
                                 ptx::f2_unpack(ptx::ffma2(ptx::f2_pack(__uint_as_float(sv[c][i]), __uint_as_float(sv[c][i + 1])), sc2, b2.x), s0, s1);
                                 ptx::f2_unpack(ptx::ffma2(ptx::f2_pack(__uint_as_float(sv[c][i + 2]), __uint_as_float(sv[c][i + 3])), sc2, b2.y), s2, s3);
@@ -833,15 +876,19 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                             for (int i = 0; i < 32; i += 2)
                                 mx4[(i >> 1) & 3] = ptx::max3(mx4[(i >> 1) & 3], __uint_as_float(sv[c][i]), __uint_as_float(sv[c][i + 1]));
                     } else {
+                        // bit i of seen: key c * 32 + i of the tile is in [lo_r, hi_r)
                         const int lo = lo_r - key_base - t * 128, hi = hi_r - key_base - t * 128;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
+                        for (int c = 0; c < 4; ++c) {
+                            const int a = min(max(lo - c * 32, 0), 32), b = min(max(hi - c * 32, 0), 32);
+                            const uint32_t seen = (uint32_t)((1ull << b) - 1) & ~(uint32_t)((1ull << a) - 1);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
-                                const float s = (c * 32 + i >= lo && c * 32 + i < hi) ? __uint_as_float(sv[c][i]) : -INFINITY;
+                                const float s = seen & (1u << i) ? __uint_as_float(sv[c][i]) : -INFINITY;
                                 sv[c][i] = __float_as_uint(s);
                                 mx4[i & 3] = fmaxf(mx4[i & 3], s);
                             }
+                        }
                     }
                     const float m_tile = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
                     // the reference moves when the maximum outgrows it by 2^8 (from -inf: at once)
@@ -854,26 +901,27 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                     }
                     const float nb = m_used == -INFINITY ? 0.f : -m_used;
                     const bool moved = __any_sync(0xffffffffu, need && old != -INFINITY);
-                    if (FOG == kValueFog && weighted) l += softmax_p<BF16, true>(sv, sreg, scale, nb, wts);
-                    else l += softmax_p<BF16, false>(sv, sreg, scale, nb, wts);
-                    // O moves with the reference (rare): its last product is complete, the next waits for p_full
+                    // O moves with the reference (rare): its last product is complete, the next waits for P
                     if (moved) {
                         const float f = need && old != -INFINITY ? ptx::ex2(old - m_used) : 1.f;
 #pragma unroll 1
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t ov[32];
-                            ptx::tmem_ld32(oreg + x * 128 + c * 32, ov);
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t ov[16];
+                            tmem_ld16(oreg + x * 128 + c * 16, ov);
                             ptx::tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
-                            ptx::tmem_st32(oreg + x * 128 + c * 32, ov);
+                            for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
+                            ptx::tmem_st16(oreg + x * 128 + c * 16, ov);
                         }
                         ptx::tmem_st_wait();
                     }
+                    if (FOG == kValueFog && weighted) l += softmax_p<BF16, true>(sv, sreg, scale, nb, wts, &ph_full[x]);
+                    else l += softmax_p<BF16, false>(sv, sreg, scale, nb, wts, &ph_full[x]);
                     ptx::tc_fence_before();
                 }
                 __syncwarp();
                 if (lane == 0) {
+                    if (!any) ptx::mbar_arrive(&ph_full[x]);
                     ptx::mbar_arrive(&p_full[x]);
                     if (weighted) mbar_arrive_n(&w_empty[wi], single ? 2 : 1);
                 }
@@ -968,6 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
 // that ends the tile; they are joined in that order.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) fog_chunks_merge_kernel(const ChunkParams p, int ctas) {
+    ptx::grid_dependency_wait();
     const PieceDesc* desc = reinterpret_cast<const PieceDesc*>(p.ws);
     const int c = blockIdx.x + 1;
     const PieceDesc d = desc[c];
@@ -1054,6 +1103,10 @@ CUresult encode_kv(CUtensorMap* map, const void* base, bool bf16, int D, int64_t
     return encode_tiled_5d_sw128(map, base, bf16, dims, str, bx);
 }
 
+size_t chunks_workspace_bytes(int head_dim) {
+    return (size_t)sm_count() * (sizeof(PieceDesc) + 2 * ((size_t)256 * head_dim * 4 + 256 * 8));
+}
+
 template <int D, bool BF16, int FOG>
 int launch_chunks(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ChunkParams& p, int grid, cudaStream_t st) {
     auto kern = fog_chunks_kernel<D, BF16, FOG>;
@@ -1073,7 +1126,23 @@ int launch_chunks(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap&
     kern<<<grid, kThreads, Cfg<D>::kAlloc, st>>>(q, k, v, p);
     const int rc = check_launch("paged_fog_chunks");
     if (rc || grid < 2) return rc;
-    fog_chunks_merge_kernel<D, BF16><<<dim3(grid - 1, 8), 256, 0, st>>>(p, grid);
+    // The merge is a programmatic dependent of the kernel above (its launch
+    // overlaps that one's run; it reads nothing before its wait).  It signals
+    // nothing early itself, and is on record for a programmatic launch behind it.
+    const ByteRange wrote[2] = {byte_span(p.o, 2 * ((int64_t)(p.T - 1) * p.o_st + (int64_t)(p.Hkv * p.G - 1) * p.o_sh + D)),
+                                byte_span(p.ws, (int64_t)chunks_workspace_bytes(D))};
+    LaunchOrderGuard order;
+    claim_early_reads(st, nullptr, 0, wrote, 2);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid - 1, 8);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, fog_chunks_merge_kernel<D, BF16>, p, grid);
     return check_launch("paged_fog_chunks merge");
 }
 
@@ -1091,7 +1160,7 @@ using namespace kessie;
 
 extern "C" size_t kessie_paged_fog_chunks_workspace_size(int num_q_heads, int num_kv_heads, int head_dim) {
     if (num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0) return 0;
-    return (size_t)sm_count() * (sizeof(PieceDesc) + 2 * ((size_t)256 * head_dim * 4 + 256 * 8));
+    return chunks_workspace_bytes(head_dim);
 }
 
 extern "C" int kessie_paged_fog_chunks_v2(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,

@@ -21,6 +21,7 @@
 #include "common.cuh"
 
 #include <math.h>
+#include <string.h>
 
 namespace kessie {
 namespace {
@@ -223,12 +224,23 @@ int launch_rope_axes(RopeAxesParams& p, const RopeAxesTable& tab, cudaStream_t s
 }
 
 int run_rope_axes(RopeAxesParams& p, int dtype, const int* sections, int interleaved, float theta, cudaStream_t st) {
-    RopeAxesTable tab{};
     if (p.axes < 1 || p.axes > kRaMaxAxes || !sections)
         return set_error(KESSIE_ERR_ARG, "rope_axes: %d axes (1 to %d)", p.axes, kRaMaxAxes);
     if (!(theta > 0.f) || isinf(theta)) return set_error(KESSIE_ERR_ARG, "rope_axes: theta %g", (double)theta);
-    const int rc = fill_table(&tab, sections, p.axes, interleaved, theta, &p.half);
-    if (rc) return rc;
+    // The table of the thread's last call is kept: a model uses one, and 64
+    // powers and remainders cost more host time than the launch.
+    struct Last { int axes = 0, sections[kRaMaxAxes], interleaved, half; float theta; RopeAxesTable tab; };
+    static thread_local Last last;
+    if (last.axes != p.axes || last.interleaved != interleaved || last.theta != theta ||
+        memcmp(last.sections, sections, p.axes * sizeof(int)) != 0) {
+        last.axes = 0;
+        const int rc = fill_table(&last.tab, sections, p.axes, interleaved, theta, &last.half);
+        if (rc) return rc;
+        last.axes = p.axes; last.interleaved = interleaved; last.theta = theta;
+        memcpy(last.sections, sections, p.axes * sizeof(int));
+    }
+    const RopeAxesTable& tab = last.tab;
+    p.half = last.half;
     if (2 * p.half > p.D) return set_error(KESSIE_ERR_ARG, "rope_axes: %d rotated dimensions of %d", 2 * p.half, p.D);
     p.status = device_status_ptr();
     if (p.T == 0) { clear_error(); return KESSIE_OK; }

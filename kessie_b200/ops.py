@@ -566,18 +566,14 @@ class StepTables(NamedTuple):
     pages_used: torch.Tensor         # int32 [1]
 
 
-def _same_device(name: str, dev: torch.device, *ts):
+def _one_device(name: str, *ts) -> int:
+    """The index of the one CUDA device that holds every tensor in ts."""
+    index = ts[0].get_device()
     for t in ts:
-        if torch.is_tensor(t) and t.device != dev:
-            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
-
-
-def _step_output(name: str, t: Optional[torch.Tensor], n: int, dtype, device) -> torch.Tensor:
-    if t is None:
-        return torch.empty(n, dtype=dtype, device=device)
-    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"step_tables: {name} must be a contiguous {dtype} tensor of {n} elements")
-    return t
+        if t is not None and t.get_device() != index or index < 0:
+            where = {str(x.device) for x in ts if x is not None}
+            raise ValueError(f"{name}: tensors must be on one CUDA device, got {', '.join(sorted(where))}")
+    return index
 
 
 def step_tables(context_lens: torch.Tensor, query_lens: torch.Tensor, block_table: torch.Tensor, page_size: int,
@@ -598,58 +594,68 @@ def step_tables(context_lens: torch.Tensor, query_lens: torch.Tensor, block_tabl
     bounds the page ids.  `out` reuses an earlier result's tensors.  Lengths
     that do not fit are cut and recorded in the device status
     (read_device_status), with -1 for the pages and slots concerned."""
-    _need_cuda(context_lens, query_lens, block_table, free_pages, free_count)
+    index = _one_device("step_tables", block_table, context_lens, query_lens, free_pages, free_count, *(out or ()))
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return step_tables(context_lens, query_lens, block_table, page_size, free_pages, num_tokens, num_pages,
+                               free_count, out, stream)
     dev = block_table.device
-    _same_device("step_tables", dev, context_lens, query_lens, free_pages, free_count, *(out or ()))
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
             (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise ValueError("step_tables: block_table must be int32 [R, maxP] with contiguous rows (it is updated in place)")
-    R = block_table.shape[0]
+    R, max_pages = block_table.shape
+    num_tokens = int(num_tokens)
     if context_lens.numel() != R or query_lens.numel() != R:
         raise ValueError("step_tables: one context and one query length per row of block_table")
-    ctx, new, free = (_i32(t, dev) for t in (context_lens, query_lens, free_pages))
-    if free_count is not None:
-        if free_count.numel() != 1:
-            raise ValueError("step_tables: free_count has one element")
-        free_count = _i32(free_count, dev)
-    shapes = (("query_start_loc", R + 1, torch.int32), ("seq_lens", R, torch.int32),
-              ("positions", int(num_tokens), torch.int32), ("slot_mapping", int(num_tokens), torch.int64),
-              ("pages_used", 1, torch.int32))
+    if free_count is not None and free_count.numel() != 1:
+        raise ValueError("step_tables: free_count has one element")
     if num_tokens < 0:
         raise ValueError("step_tables: num_tokens must not be negative")
-    res = StepTables(*(_step_output(name, getattr(out, name) if out is not None else None, n, dt, dev)
-                       for name, n, dt in shapes))
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().kessie_step_tables_v2(
-            _p(ctx), _p(new), R, _p(block_table), block_table.stride(0), block_table.shape[1], int(page_size),
-            2 ** 31 - 1 if num_pages is None else int(num_pages), _p(free), free.numel(), _p(free_count),
-            int(num_tokens), *(_p(t) for t in res), _stream(stream, dev.index)), "step_tables")
+    ctx, new, free, count = (_i32(t, dev) for t in (context_lens, query_lens, free_pages, free_count))
+    if out is None:
+        # one allocation for the int32 outputs
+        flat = torch.empty(2 * R + 2 + num_tokens, dtype=torch.int32, device=dev)
+        res = StepTables(flat.narrow(0, 0, R + 1), flat.narrow(0, R + 1, R), flat.narrow(0, 2 * R + 2, num_tokens),
+                         torch.empty(num_tokens, dtype=torch.int64, device=dev), flat.narrow(0, 2 * R + 1, 1))
+    else:
+        res = out
+        for name, t, n, dt in zip(StepTables._fields, out, (R + 1, R, num_tokens, num_tokens, 1),
+                                  (torch.int32, torch.int32, torch.int32, torch.int64, torch.int32)):
+            if t.dtype != dt or t.numel() != n or not t.is_contiguous():
+                raise ValueError(f"step_tables: {name} must be a contiguous {dt} tensor of {n} elements")
+    _lib.check(_lib.load().kessie_step_tables_v2(
+        ctx.data_ptr(), new.data_ptr(), R, block_table.data_ptr(), block_table.stride(0), max_pages, int(page_size),
+        2 ** 31 - 1 if num_pages is None else int(num_pages), free.data_ptr(), free.numel(), _p(count), num_tokens,
+        res.query_start_loc.data_ptr(), res.seq_lens.data_ptr(), res.positions.data_ptr(), res.slot_mapping.data_ptr(),
+        res.pages_used.data_ptr(), _stream(stream, index)), "step_tables")
     return res
 
 
 def _axis_positions(name: str, positions, axes: int, tokens: int, device) -> torch.Tensor:
     t = positions if torch.is_tensor(positions) else torch.as_tensor(positions, device=device)
-    if t.dim() == 1 and axes == 1:
+    if axes == 1 and t.dim() == 1:
         t = t.unsqueeze(0)
     if t.shape != (axes, tokens):
         raise ValueError(f"{name}: positions must be [{axes}, {tokens}], one row per axis, got {tuple(t.shape)}")
-    _need_cuda(t)
+    if t.device != device:
+        raise ValueError(f"{name}: positions must be on {device}, got {t.device}")
     if t.dtype != torch.int32:
         t = t.to(torch.int32)
-    return t if t.stride(1) == 1 or tokens <= 1 else t.contiguous()
+    return t if tokens <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
 def _sections(name: str, sections: Sequence[int]):
-    sec = [int(x) for x in sections]
-    if not sec:
+    n = len(sections)
+    if n == 0:
         raise ValueError(f"{name}: sections must give each axis its number of frequencies")
-    return (ctypes.c_int * len(sec))(*sec), len(sec)
+    return (ctypes.c_int * n)(*sections), n
 
 
 def _rows(name: str, x: torch.Tensor):
-    if x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
+    st = x.stride()
+    if len(st) != 3 or (st[2] != 1 and x.shape[2] > 1):
         raise ValueError(f"{name}: rows must be [tokens, heads, head_dim] with head_dim contiguous")
-    return x.stride(0), x.stride(1)
+    return st
 
 
 def rope_axes_remap(k: torch.Tensor, orig_positions, target_positions, sections: Sequence[int],
@@ -663,8 +669,11 @@ def rope_axes_remap(k: torch.Tensor, orig_positions, target_positions, sections:
     d % axes while d < axes * sections[axis], else to the first).  With
     orig_positions None the keys are rotated from position 0.  Angles are
     exact to fp32 at any int32 position."""
-    _need_cuda(k, out)
     out = k if out is None else out
+    index = _one_device("rope_axes_remap", k, out)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return rope_axes_remap(k, orig_positions, target_positions, sections, rope_theta, interleaved, out, stream)
     if out.shape != k.shape or out.dtype != k.dtype:
         raise ValueError("rope_axes_remap: out must match k's shape and dtype")
     T, H, D = k.shape
@@ -672,12 +681,10 @@ def rope_axes_remap(k: torch.Tensor, orig_positions, target_positions, sections:
     sec, axes = _sections("rope_axes_remap", sections)
     tgt = _axis_positions("rope_axes_remap", target_positions, axes, T, k.device)
     org = None if orig_positions is None else _axis_positions("rope_axes_remap", orig_positions, axes, T, k.device)
-    _same_device("rope_axes_remap", k.device, out, tgt, org)
-    with torch.cuda.device(k.device):
-        _lib.check(_lib.load().kessie_rope_axes_remap_v2(
-            _p(k), *ks, _p(out), *os_, dtype_code(k), T, H, D, _p(org), org.stride(0) if org is not None else 0,
-            _p(tgt), tgt.stride(0), sec, axes, 1 if interleaved else 0, float(rope_theta),
-            _stream(stream, k.device.index)), "rope_axes_remap")
+    _lib.check(_lib.load().kessie_rope_axes_remap_v2(
+        k.data_ptr(), ks[0], ks[1], out.data_ptr(), os_[0], os_[1], dtype_code(k), T, H, D, _p(org),
+        org.stride(0) if org is not None else 0, tgt.data_ptr(), tgt.stride(0), sec, axes, 1 if interleaved else 0,
+        float(rope_theta), _stream(stream, index)), "rope_axes_remap")
     return out
 
 
@@ -691,11 +698,16 @@ def rope_axes_insert(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, position
     (layout as in page_insert) that slot_mapping (int64 [T], page * page_size +
     token; negative: not written) names.  Sections and angles as in
     rope_axes_remap; slots must be distinct.  One launch."""
-    _need_cuda(q, k, v, kv, slot_mapping, out_q)
     out_q = q if out_q is None else out_q
+    index = _one_device("rope_axes_insert", q, k, v, kv, slot_mapping, out_q)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return rope_axes_insert(q, k, v, positions, sections, kv, slot_mapping, rope_theta, interleaved, out_q,
+                                    layout, stream)
     T, Hq, D = q.shape
     ps_, ts_, kvs_, hs_, P, ps, Hkv, Dc = kv_layout_strides(kv, layout)
-    if k.shape != (T, Hkv, D) or v.shape != k.shape or Dc != D or out_q.shape != q.shape:
+    rows = (T, Hkv, D)
+    if k.shape != rows or v.shape != rows or Dc != D or out_q.shape != q.shape:
         raise ValueError(f"rope_axes_insert: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, "
                          f"out_q {tuple(out_q.shape)} do not match a cache of {Hkv} heads of {Dc}")
     if not (q.dtype == k.dtype == v.dtype == kv.dtype == out_q.dtype):
@@ -707,13 +719,13 @@ def rope_axes_insert(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, position
     qs, ks, vs, os_ = (_rows("rope_axes_insert", x) for x in (q, k, v, out_q))
     sec, axes = _sections("rope_axes_insert", sections)
     pos = _axis_positions("rope_axes_insert", positions, axes, T, q.device)
-    _same_device("rope_axes_insert", q.device, k, v, kv, slot_mapping, out_q, pos)
-    slots = slot_mapping.to(torch.int64).contiguous()
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.load().kessie_rope_axes_insert_v2(
-            _p(q), *qs, _p(out_q), *os_, _p(k), *ks, _p(v), *vs, dtype_code(q), T, Hq, Hkv, D, _p(pos), pos.stride(0),
-            sec, axes, 1 if interleaved else 0, float(rope_theta), _p(kv), ps_, ts_, kvs_, hs_, P, ps, _p(slots),
-            _stream(stream, q.device.index)), "rope_axes_insert")
+    slots = slot_mapping if slot_mapping.dtype == torch.int64 else slot_mapping.to(torch.int64)
+    slots = slots.contiguous()
+    _lib.check(_lib.load().kessie_rope_axes_insert_v2(
+        q.data_ptr(), qs[0], qs[1], out_q.data_ptr(), os_[0], os_[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
+        vs[1], dtype_code(q), T, Hq, Hkv, D, pos.data_ptr(), pos.stride(0), sec, axes, 1 if interleaved else 0,
+        float(rope_theta), kv.data_ptr(), ps_, ts_, kvs_, hs_, P, ps, slots.data_ptr(), _stream(stream, index)),
+        "rope_axes_insert")
     return out_q
 
 
@@ -736,21 +748,26 @@ def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     Returns out [T, Hq, D]; rows that see no key are 0, rows of no sequence (a
     padded batch) are not written.  Scratch memory: one buffer per stream, a
     graph capture gets its own; or `ws` (chunks_workspace_bytes() bytes)."""
-    _need_cuda(q, k_cache, v_cache, block_table, query_start_loc, seq_lens, out)
+    index = _one_device("paged_fog_chunks", q, k_cache, v_cache, block_table, query_start_loc, seq_lens, out, ws)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return paged_fog_chunks(q, k_cache, v_cache, block_table, query_start_loc, seq_lens, clear_start, fog_alpha,
+                                    window_size, causal, sm_scale, max_seq_len, out, stream, ws, bias)
     T, Hq, D = q.shape
     P, ps, Hkv, Dk = k_cache.shape
-    ks = k_cache.stride()
+    ks, qs = k_cache.stride(), q.stride()
     if Dk != D or v_cache.shape != k_cache.shape or v_cache.stride() != ks:
         raise ValueError("k_cache/v_cache must be matching [P, ps, Hkv, D] views")
     if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
         raise TypeError("q and the cache must share a dtype")
     if ks[3] != 1:
         raise ValueError("head_dim must be contiguous")
-    B = block_table.shape[0]
+    B, width = block_table.shape
     if query_start_loc.numel() != B + 1 or seq_lens.numel() != B:
         raise ValueError("paged_fog_chunks: block_table [B, maxP], query_start_loc [B + 1], seq_lens [B]")
-    if q.stride(2) != 1 or (q.stride(0) | q.stride(1)) % 8 or q.data_ptr() % 16:
+    if qs[2] != 1 or (qs[0] | qs[1]) % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)      # rows the kernel cannot load: a copy
+        qs = q.stride()
     if out is None:
         out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
@@ -759,27 +776,28 @@ def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     bt = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
     if bt.stride(1) != 1:
         bt = bt.contiguous()
-    qsl, sl, cs = _i32(query_start_loc, dev), _i32(seq_lens, dev), _i32(clear_start, dev)
-    _same_device("paged_fog_chunks", dev, k_cache, v_cache, bt, qsl, sl, cs, out)
-    cap = bt.shape[1] * ps
+    qsl, sl = _i32(query_start_loc, dev), _i32(seq_lens, dev)
+    cs = _i32(clear_start, dev)
+    if cs is not None and (cs.numel() != B or cs.get_device() != index):
+        raise ValueError("paged_fog_chunks: clear_start has one entry per sequence, on q's device")
+    cap = width * ps
     if max_seq_len is None:
         max_seq_len = cap
-    if max_seq_len > cap:
+    elif max_seq_len > cap:
         raise ValueError(f"max_seq_len {max_seq_len} exceeds the block table capacity {cap}")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
     lib = _lib.load()
-    cb = bias.c_struct() if bias is not None else None
-    with torch.cuda.device(dev):
-        handle = _stream(stream, dev.index)
-        if ws is None:
-            ws = _stream_workspace(lib.kessie_paged_fog_chunks_workspace_size(Hq, Hkv, D), dev, "chunks", handle)
-        _lib.check(lib.kessie_paged_fog_chunks_v2(
-            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], P, ps,
-            bt.data_ptr(), bt.stride(0), qsl.data_ptr(), sl.data_ptr(), _p(cs), float(fog_alpha), int(window_size),
-            1 if causal else 0, float(sm_scale), B, T, Hq, Hkv, D, int(max_seq_len), dtype_code(q),
-            ctypes.byref(cb) if cb is not None else None, out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr(),
-            ws.numel(), handle), "paged_fog_chunks")
+    handle = _stream(stream, index)
+    if ws is None:
+        ws = _stream_workspace(lib.kessie_paged_fog_chunks_workspace_size(Hq, Hkv, D), dev, "chunks", handle)
+    os_ = out.stride()
+    _lib.check(lib.kessie_paged_fog_chunks_v2(
+        q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], P, ps, bt.data_ptr(),
+        bt.stride(0), qsl.data_ptr(), sl.data_ptr(), _p(cs), float(fog_alpha), int(window_size), 1 if causal else 0,
+        float(sm_scale), B, T, Hq, Hkv, D, int(max_seq_len), dtype_code(q),
+        None if bias is None else ctypes.byref(bias.c_struct()), out.data_ptr(), os_[0], os_[1], ws.data_ptr(),
+        ws.numel(), handle), "paged_fog_chunks")
     return out
 
 
