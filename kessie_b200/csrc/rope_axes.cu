@@ -10,23 +10,34 @@
 //
 // Angles.  Positions reach 10^6 and f_0 = 1, so an fp32 product would be off
 // by up to 0.06 rad.  The host stores F_d = frac(f_d / 2 pi) as a 64-bit
-// fixed-point fraction of a turn; the integer product delta * F_d mod 2^64 is
-// the angle's fraction of a turn, off by less than |delta| * 2^-64 turns, with
-// no range reduction; sincospif takes it from there (fp32, ~1e-7 rad).
+// fixed-point fraction of a turn; position * F_d mod 2^64 is the angle's
+// fraction of a turn, off by less than |position| * 2^-64 turns, with no range
+// reduction, and its top 32 bits are kept.  For fp32 rows sincospif takes it
+// from there (~1e-7); for 16-bit rows the hardware sine and cosine on [-pi, pi]
+// do (absolute error below 5e-7, against 2^-12 of the stored rounding).
 //
-// HBM-bound: every row is read and written once (16 bytes a lane and access).
-// A warp takes one token: its lanes compute the token's cos / sin once into
-// shared memory, each keeps those of its own vector in registers, and then
-// runs through the q, k and v rows, 32 / (half / VEC) rows at a time.
+// HBM-bound: every row is read and written once (16 bytes a thread and access).
+// A thread owns one vector pair (VEC neighbouring frequencies) of one token and
+// runs through the token's q, k and v heads, kRaBatch of them in flight: the
+// token's angles are computed once over its threads, stay in registers, and
+// nothing is shared.  Forms that shared angles through shared memory (a warp or
+// a CTA per block of tokens) issued 500 to 570 instructions a token for the remap
+// of 65,536 keys of 8 fp16 heads and took 55 to 76 us; this one takes 45.3 us,
+// 230 instructions a token (5.96 TB/s; a plain copy of the same bytes: 44 us).
+// 8,197 new tokens of 32 + 8 + 8 bf16 heads into their slots: 38 us, 5.3 TB/s.
 #include "common.cuh"
+#include "ptx.cuh"
 
+#include <limits.h>
 #include <math.h>
 #include <string.h>
 
 namespace kessie {
 namespace {
 
-constexpr int kRaWarps = 8;
+constexpr int kRaThreads = 64;
+constexpr int kRaBatch = 4;                // heads in flight per thread
+constexpr int kRaWarps = 8;                // warps an SM wanted before threads take whole tokens
 constexpr int kRaMaxHalf = 256;
 constexpr int kRaMaxAxes = 8;
 
@@ -47,19 +58,13 @@ struct RopeAxesParams {
     void* kv; int64_t page_stride, token_stride, kv_stride, head_stride;
     int64_t num_slots;
     int page_size;
-    int iters;                      // row groups per work item
-    int chunks;                     // work items per token
+    int rows, parts;                // rows (of Hq + 2 Hkv) that a thread takes, threads per vector pair and token
     int* status;
 };
 
-template <typename T, int VEC> struct RaVec;
-template <typename T> struct RaVec<T, 1> {
-    T x[1];
-    __device__ void load(const T* p) { x[0] = *p; }
-    __device__ void store(T* p) const { *p = x[0]; }
-};
-template <typename T, int VEC> struct alignas(16) RaVec {
-    T x[VEC];
+template <typename T> struct alignas(16) RaVec {
+    static constexpr int N = 16 / sizeof(T);
+    T x[N];
     __device__ void load(const T* p) {
         uint4 u;
         asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -69,89 +74,206 @@ template <typename T, int VEC> struct alignas(16) RaVec {
     __device__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(x); }
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ void ra_rotate(RaVec<T, VEC>& lo, RaVec<T, VEC>& hi, const float2* cs) {
+template <typename T>
+__device__ __forceinline__ void ra_rotate(T& lo, T& hi, float2 cs) {
+    const float a = to_f32(lo), b = to_f32(hi);
+    lo = from_f32<T>(a * cs.x - b * cs.y);                     // one rounding to the stored type
+    hi = from_f32<T>(a * cs.y + b * cs.x);
+}
+
+// Two neighbouring elements as a packed fp32 pair, and back (one rounding).
+__device__ __forceinline__ uint64_t ra_load2(const __half* x) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(x));
+    return ptx::f2_pack(f.x, f.y);
+}
+__device__ __forceinline__ uint64_t ra_load2(const __nv_bfloat16* x) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(x));
+    return ptx::f2_pack(f.x, f.y);
+}
+__device__ __forceinline__ uint64_t ra_load2(const float* x) { return ptx::f2_pack(x[0], x[1]); }
+__device__ __forceinline__ void ra_store2(__half* x, uint64_t v) {
+    float a, b;
+    ptx::f2_unpack(v, a, b);
+    *reinterpret_cast<__half2*>(x) = __floats2half2_rn(a, b);
+}
+__device__ __forceinline__ void ra_store2(__nv_bfloat16* x, uint64_t v) {
+    float a, b;
+    ptx::f2_unpack(v, a, b);
+    *reinterpret_cast<__nv_bfloat162*>(x) = __floats2bfloat162_rn(a, b);
+}
+__device__ __forceinline__ void ra_store2(float* x, uint64_t v) { ptx::f2_unpack(v, x[0], x[1]); }
+
+// Rotate elements x[0], x[1] of both halves; cs = (cos, cos, sin, sin).
+template <typename T>
+__device__ __forceinline__ void ra_rotate2(T* lo, T* hi, float4 cs) {
+    const uint64_t a = ra_load2(lo), b = ra_load2(hi);
+    const uint64_t c = ptx::f2_pack(cs.x, cs.y), s = ptx::f2_pack(cs.z, cs.w), ns = ptx::f2_pack(-cs.z, -cs.w);
+    ra_store2(lo, ptx::ffma2(a, c, ptx::fmul2(b, ns)));
+    ra_store2(hi, ptx::ffma2(a, s, ptx::fmul2(b, c)));
+}
+
+// cos and sin of a signed fraction of a turn in units of 2^-32.
+template <bool EXACT>
+__device__ __forceinline__ float2 ra_cos_sin(int32_t turn) {
+    float s, c;
+    if (EXACT) sincospif((float)turn * 0x1p-31f, &s, &c);
+    else __sincosf((float)turn * (3.14159265358979f * 0x1p-31f), &s, &c);
+    return make_float2(c, s);
+}
+
+// Top 32 bits of position * turn mod 2^64.
+__device__ __forceinline__ uint32_t ra_turns(uint64_t turn, int position) {
+    const uint32_t lo = (uint32_t)turn, hi = (uint32_t)(turn >> 32), u = (uint32_t)position;
+    return __umulhi(lo, u) + hi * u - (position < 0 ? lo : 0u);
+}
+// cos and sin of the move from orig to target (each product's truncation: 2^-32 turns).
+template <typename T>
+__device__ __forceinline__ float2 ra_angle(uint64_t turn, int target, int orig) {
+    return ra_cos_sin<sizeof(T) == 4>((int32_t)(ra_turns(turn, target) - ra_turns(turn, orig)));
+}
+// Element offset of slot's row in the cache, or -1 (not written; bad: past the cache).
+__device__ __forceinline__ int64_t ra_cache_row(const RopeAxesParams& p, int64_t slot, bool& bad) {
+    if (slot < 0) return -1;
+    if (slot >= p.num_slots) { bad = true; return -1; }
+    const int64_t page = slot <= 0x7fffffff ? (int64_t)((uint32_t)slot / (uint32_t)p.page_size) : slot / p.page_size;
+    return page * p.page_stride + (slot - page * p.page_size) * p.token_stride;
+}
+
+// Vector pairs of kRaBatch heads (of the n from src on).
+template <typename T> struct RaHeads {
+    RaVec<T> lo[kRaBatch], hi[kRaBatch];
+    __device__ __forceinline__ void load(const T* src, int64_t sh, int n, int half) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        const float a = to_f32(lo.x[i]), b = to_f32(hi.x[i]);
-        lo.x[i] = from_f32<T>(a * cs[i].x - b * cs[i].y);       // one rounding to the stored type
-        hi.x[i] = from_f32<T>(a * cs[i].y + b * cs[i].x);
+        for (int u = 0; u < kRaBatch; ++u)
+            if (u < n) {
+                lo[u].load(src + u * sh);
+                hi[u].load(src + u * sh + half);
+            }
+    }
+};
+// n heads from src to dst, rotated (or copied) by this thread's angles; the
+// first kRaBatch are in x already.
+template <bool TURN, typename T>
+__device__ __forceinline__ void ra_heads(RaHeads<T>& x, const T* src, int64_t sh, T* dst, int64_t dh, int n, int half,
+                                         const float4 (&cs)[RaVec<T>::N / 2]) {
+    while (true) {
+#pragma unroll
+        for (int u = 0; u < kRaBatch; ++u)
+            if (u < n) {
+                if (TURN)
+#pragma unroll
+                    for (int e = 0; e < RaVec<T>::N / 2; ++e) ra_rotate2(&x.lo[u].x[2 * e], &x.hi[u].x[2 * e], cs[e]);
+                x.lo[u].store(dst + u * dh);
+                x.hi[u].store(dst + u * dh + half);
+            }
+        n -= kRaBatch;
+        if (n <= 0) break;
+        src += kRaBatch * sh;
+        dst += kRaBatch * dh;
+        x.load(src, sh, n, half);
     }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kRaWarps * 32) rope_axes_kernel(const __grid_constant__ RopeAxesParams p,
-                                                                  const __grid_constant__ RopeAxesTable tab) {
-    extern __shared__ __align__(16) uint8_t ra_smem[];
-    uint64_t* turn = reinterpret_cast<uint64_t*>(ra_smem);
-    float2* cs_all = reinterpret_cast<float2*>(turn + p.half);
-    uint8_t* axis = reinterpret_cast<uint8_t*>(cs_all + kRaWarps * p.half);
-    for (int d = threadIdx.x; d < p.half; d += blockDim.x) {
+template <typename T>
+__global__ void __launch_bounds__(kRaThreads) rope_axes_kernel(const __grid_constant__ RopeAxesParams p,
+                                                               const __grid_constant__ RopeAxesTable tab) {
+    constexpr int VEC = RaVec<T>::N;
+    __shared__ uint64_t turn[kRaMaxHalf];
+    __shared__ uint8_t axis[kRaMaxHalf];
+    const int npair = p.half / VEC;                               // threads per token
+    const int per_cta = kRaThreads / npair;
+    const int sub = threadIdx.x / npair, vec = threadIdx.x - sub * npair, off = vec * VEC;
+    const int64_t item = (int64_t)blockIdx.x * per_cta + sub;     // (token, part of its rows)
+    const int64_t t = p.parts == 1 ? item : item / p.parts;
+    const int part = (int)(item - t * p.parts);
+    const bool on = sub < per_cta && t < p.T;
+    // rows [r0, r1) of q heads, k heads, v heads: heads [q0, q1), [k0, k1), [v0, v1)
+    const int r0 = part * p.rows, r1 = on ? min(r0 + p.rows, p.Hq + 2 * p.Hkv) : r0;
+    const int q0 = r0, q1 = min(r1, p.Hq), k0 = max(r0 - p.Hq, 0), k1 = min(r1 - p.Hq, p.Hkv);
+    const int v0 = max(r0 - p.Hq - p.Hkv, 0), v1 = r1 - p.Hq - p.Hkv;
+    const T* q = static_cast<const T*>(p.q) + t * p.q_st + q0 * p.q_sh + off;
+    const T* k = static_cast<const T*>(p.k) + t * p.k_st + k0 * p.k_sh + off;
+    const T* v = static_cast<const T*>(p.v) + t * p.v_st + v0 * p.v_sh + off;
+    // the first rows are on their way while the angles are computed
+    RaHeads<T> x;
+    if (q0 < q1) x.load(q, p.q_sh, q1 - q0, p.half);
+    else if (k0 < k1) x.load(k, p.k_sh, k1 - k0, p.half);
+    for (int d = threadIdx.x; d < p.half; d += kRaThreads) {
         turn[d] = tab.turn[d];
         axis[d] = tab.axis[d];
     }
     __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float2* cs = cs_all + warp * p.half;
-    const int npair = p.half / VEC;                               // vectors per half row (<= 32 when VEC > 1)
-    const int rpi = VEC > 1 ? 32 / npair : 1;                     // rows per warp step
-    const int sub = VEC > 1 ? lane / npair : 0;
-    const int rows = p.Hq + 2 * p.Hkv;
-    const int64_t items = (int64_t)p.T * p.chunks;
-    bool bad = false;
-    for (int64_t it = (int64_t)blockIdx.x * kRaWarps + warp; it < items; it += (int64_t)gridDim.x * kRaWarps) {
-        const int t = (int)(it / p.chunks), chunk = (int)(it - (int64_t)t * p.chunks);
-        __syncwarp();
-        for (int d = lane; d < p.half; d += 32) {
-            const int a = axis[d];
-            int64_t delta = p.target[a * p.target_sa + t];
-            if (p.orig) delta -= p.orig[a * p.orig_sa + t];
-            const int32_t half_turns = (int32_t)(((uint64_t)delta * turn[d] + (1ull << 31)) >> 32);
-            float s, c;
-            sincospif((float)half_turns * 0x1p-31f, &s, &c);
-            cs[d] = make_float2(c, s);
-        }
-        __syncwarp();
-        float2 mine[VEC > 1 ? VEC : 1];
-        if (VEC > 1) {
+    if (r0 >= r1) return;
+    float4 cs[VEC / 2];                                           // (cos, cos, sin, sin) of two dimensions
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) mine[i] = cs[min((lane - sub * npair) * VEC + i, p.half - 1)];
+    for (int e = 0; e < VEC / 2; ++e) {
+        float2 a2[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int d = off + 2 * e + i, a = axis[d];
+            a2[i] = ra_angle<T>(turn[d], __ldg(p.target + a * p.target_sa + t), p.orig ? __ldg(p.orig + a * p.orig_sa + t) : 0);
         }
-        int64_t cache_row = -1;
-        if (p.Hkv) {
-            const int64_t slot = p.slots[t];
-            if (slot >= p.num_slots) bad = true;
-            else if (slot >= 0) cache_row = (slot / p.page_size) * p.page_stride + (slot % p.page_size) * p.token_stride;
+        cs[e] = make_float4(a2[0].x, a2[1].x, a2[0].y, a2[1].y);
+    }
+    bool bad = false;
+    const int64_t row = r1 > p.Hq ? ra_cache_row(p, p.slots[t], bad) : -1;
+    T* kv = static_cast<T*>(p.kv) + row + off;
+    if (q0 < q1) {
+        ra_heads<true>(x, q, p.q_sh, static_cast<T*>(p.oq) + t * p.oq_st + q0 * p.oq_sh + off, p.oq_sh, q1 - q0, p.half, cs);
+        if (k0 < k1 && row >= 0) x.load(k, p.k_sh, k1 - k0, p.half);
+    }
+    if (k0 < k1 && row >= 0) ra_heads<true>(x, k, p.k_sh, kv + k0 * p.head_stride, p.head_stride, k1 - k0, p.half, cs);
+    if (v0 < v1 && row >= 0) {
+        x.load(v, p.v_sh, v1 - v0, p.half);
+        ra_heads<false>(x, v, p.v_sh, kv + p.kv_stride + v0 * p.head_stride, p.head_stride, v1 - v0, p.half, cs);
+    }
+    if (2 * p.half < p.D) {                                       // dimensions past the rotated ones
+        for (int r = r0; r < r1; ++r) {
+            const int sec = r < p.Hq ? 0 : r < p.Hq + p.Hkv ? 1 : 2, h = r - (sec == 0 ? 0 : p.Hq + (sec - 1) * p.Hkv);
+            if (sec != 0 && row < 0) break;
+            const T* src = sec == 0 ? static_cast<const T*>(p.q) + t * p.q_st + h * p.q_sh
+                         : sec == 1 ? static_cast<const T*>(p.k) + t * p.k_st + h * p.k_sh
+                                    : static_cast<const T*>(p.v) + t * p.v_st + h * p.v_sh;
+            T* dst = sec == 0 ? static_cast<T*>(p.oq) + t * p.oq_st + h * p.oq_sh
+                              : static_cast<T*>(p.kv) + row + (sec == 2 ? p.kv_stride : 0) + h * p.head_stride;
+            for (int d = 2 * p.half + off; d < p.D; d += p.half) {
+                RaVec<T> y;
+                y.load(src + d);
+                y.store(dst + d);
+            }
         }
-        const int r_end = min(rows, (chunk + 1) * p.iters * rpi);
-        for (int r = chunk * p.iters * rpi + sub; r < r_end; r += rpi) {
-            if (sub >= rpi) break;                               // lanes past the last whole row
-            const T* src;
-            T* dst;
-            if (r < p.Hq) {
-                src = static_cast<const T*>(p.q) + t * p.q_st + r * p.q_sh;
-                dst = static_cast<T*>(p.oq) + t * p.oq_st + r * p.oq_sh;
-            } else {
-                const int h = r - p.Hq, is_v = h >= p.Hkv, hh = h - is_v * p.Hkv;
-                if (cache_row < 0) continue;
-                src = is_v ? static_cast<const T*>(p.v) + t * p.v_st + hh * p.v_sh
-                           : static_cast<const T*>(p.k) + t * p.k_st + hh * p.k_sh;
-                dst = static_cast<T*>(p.kv) + cache_row + is_v * p.kv_stride + hh * p.head_stride;
-            }
-            const bool turned = r < p.Hq + p.Hkv;
-            const int first = VEC > 1 ? lane - sub * npair : lane, stride = VEC > 1 ? npair : 32;
-            for (int e = first; e < npair; e += stride) {
-                RaVec<T, VEC> lo, hi;
-                lo.load(src + e * VEC);
-                hi.load(src + p.half + e * VEC);
-                if (turned) ra_rotate<T, VEC>(lo, hi, VEC > 1 ? mine : cs + e);
-                lo.store(dst + e * VEC);
-                hi.store(dst + p.half + e * VEC);
-            }
-            for (int e = 2 * npair + first; e < p.D / VEC; e += stride) {
-                RaVec<T, VEC> x;
-                x.load(src + e * VEC);
-                x.store(dst + e * VEC);
+    }
+    if (bad) record_status(p.status, KESSIE_DEV_BAD_PAGE_ID);
+}
+
+// Rows that are not 16-byte aligned, or half not a multiple of a vector: a
+// warp per token, one element a lane.
+template <typename T>
+__global__ void __launch_bounds__(kRaThreads) rope_axes_scalar_kernel(const __grid_constant__ RopeAxesParams p,
+                                                                         const __grid_constant__ RopeAxesTable tab) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    bool bad = false;
+    for (int64_t t = (int64_t)blockIdx.x * (kRaThreads / 32) + warp; t < p.T; t += (int64_t)gridDim.x * (kRaThreads / 32)) {
+        const int64_t row = p.Hkv ? ra_cache_row(p, p.slots[t], bad) : -1;
+        for (int d = lane; d < p.D - p.half; d += 32) {              // [0, half): a pair; above: a dimension as it is
+            const int e = d < p.half ? d : d + p.half;
+            const float2 c = d < p.half ? ra_angle<T>(tab.turn[d], p.target[tab.axis[d] * p.target_sa + t],
+                                                        p.orig ? p.orig[tab.axis[d] * p.orig_sa + t] : 0) : make_float2(1.f, 0.f);
+            for (int h = 0; h < p.Hq + 2 * p.Hkv; ++h) {
+                const int sec = h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2, r = h - (sec == 0 ? 0 : p.Hq + (sec - 1) * p.Hkv);
+                if (sec != 0 && row < 0) break;
+                const T* src = sec == 0 ? static_cast<const T*>(p.q) + t * p.q_st + r * p.q_sh
+                             : sec == 1 ? static_cast<const T*>(p.k) + t * p.k_st + r * p.k_sh
+                                        : static_cast<const T*>(p.v) + t * p.v_st + r * p.v_sh;
+                T* dst = sec == 0 ? static_cast<T*>(p.oq) + t * p.oq_st + r * p.oq_sh
+                                  : static_cast<T*>(p.kv) + row + (sec == 2 ? p.kv_stride : 0) + r * p.head_stride;
+                T lo = src[e];
+                if (d < p.half) {
+                    T hi = src[e + p.half];
+                    if (sec != 2) ra_rotate(lo, hi, c);
+                    dst[e + p.half] = hi;
+                }
+                dst[e] = lo;
             }
         }
     }
@@ -192,35 +314,33 @@ int fill_table(RopeAxesTable* tab, const int* sections, int axes, int interleave
     return KESSIE_OK;
 }
 
-template <typename T, int VEC>
-int launch_typed(RopeAxesParams& p, const RopeAxesTable& tab, cudaStream_t st) {
-    const int npair = p.half / VEC;
-    const int rpi = VEC > 1 ? 32 / npair : 1;
-    const int groups = (p.Hq + 2 * p.Hkv + rpi - 1) / rpi;
-    // One warp walks all rows of a token once there are tokens for 16 warps an
-    // SM; below that the rows are spread over more warps (each redoes the
-    // token's angles), so that a decode step's few tokens still fill the GPU.
-    const int64_t want = 16LL * sm_count();
-    int64_t iters = (int64_t)p.T * groups / want;
-    p.iters = (int)(iters < 1 ? 1 : iters < groups ? iters : groups);
-    p.chunks = (groups + p.iters - 1) / p.iters;
-    const size_t smem = p.half * (sizeof(uint64_t) + kRaWarps * sizeof(float2) + 1);
-    const int64_t ctas = ((int64_t)p.T * p.chunks + kRaWarps - 1) / kRaWarps;
-    const int64_t cap = 8LL * sm_count();
-    rope_axes_kernel<T, VEC><<<(int)(ctas < cap ? ctas : cap), kRaWarps * 32, smem, st>>>(p, tab);
-    return check_launch("rope_axes");
-}
-
 template <typename T>
 int launch_rope_axes(RopeAxesParams& p, const RopeAxesTable& tab, cudaStream_t st) {
-    constexpr int VEC = 16 / sizeof(T);
-    const int64_t es = sizeof(T);
-    uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.oq) |
-                     reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | reinterpret_cast<uintptr_t>(p.kv);
-    int64_t steps = p.q_st | p.q_sh | p.oq_st | p.oq_sh | p.k_st | p.k_sh | p.v_st | p.v_sh | p.page_stride |
-                    p.token_stride | p.kv_stride | p.head_stride | p.half | p.D;
-    const bool vec = !(bits & 15) && !((steps * es) & 15) && p.half / VEC <= 32;
-    return vec ? launch_typed<T, VEC>(p, tab, st) : launch_typed<T, 1>(p, tab, st);
+    constexpr int VEC = RaVec<T>::N;
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.oq) |
+                           reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
+                           reinterpret_cast<uintptr_t>(p.kv);
+    const int64_t steps = p.q_st | p.q_sh | p.oq_st | p.oq_sh | p.k_st | p.k_sh | p.v_st | p.v_sh | p.page_stride |
+                          p.token_stride | p.kv_stride | p.head_stride | p.half | p.D;
+    const int64_t sms = sm_count();
+    if ((bits & 15) || (steps % VEC) || p.half / VEC > 32) {
+        const int64_t ctas = ((int64_t)p.T + kRaThreads / 32 - 1) / (kRaThreads / 32);
+        rope_axes_scalar_kernel<T><<<(int)(ctas < 16 * sms ? ctas : 16 * sms), kRaThreads, 0, st>>>(p, tab);
+        return check_launch("rope_axes");
+    }
+    // One thread takes all rows of its vector pair, unless that leaves less
+    // than kRaWarps warps an SM: then the rows are shared out (each thread
+    // redoes the angles), down to kRaBatch of them.
+    const int per_cta = kRaThreads / (p.half / VEC), all_rows = p.Hq + 2 * p.Hkv;
+    const int64_t warps = ((int64_t)p.T + per_cta - 1) / per_cta * (kRaThreads / 32), want = kRaWarps * sms;
+    int64_t parts = warps < want ? (want + warps - 1) / warps : 1;
+    if (parts > (all_rows + kRaBatch - 1) / kRaBatch) parts = (all_rows + kRaBatch - 1) / kRaBatch;
+    p.rows = (int)((all_rows + parts - 1) / parts);
+    p.parts = (all_rows + p.rows - 1) / p.rows;
+    const int64_t ctas = ((int64_t)p.T * p.parts + per_cta - 1) / per_cta;
+    if (ctas > INT_MAX) return set_error(KESSIE_ERR_UNSUPPORTED, "rope_axes: %d tokens", p.T);
+    rope_axes_kernel<T><<<(int)ctas, kRaThreads, 0, st>>>(p, tab);
+    return check_launch("rope_axes");
 }
 
 int run_rope_axes(RopeAxesParams& p, int dtype, const int* sections, int interleaved, float theta, cudaStream_t st) {
