@@ -7,7 +7,7 @@ once per step (``_FogCache``) and passes it to vLLM's own attention as
 so the fog never reaches the scores; the reference also sizes the bias from
 ``key.shape[-2]``, the KV-head count of vLLM's [tokens, heads, dim] keys.
 Here ``KeSSieAttentionImpl`` computes the attention itself with the paged
-decode / chunked-prefill kernels of this library, the bias applied to the
+decode and ragged-chunk kernels of this library, the bias applied to the
 scaled scores inside the kernels, per request of kv_len = its sequence
 length:
     fb = int(kv_len * (1 - fog_start))
@@ -154,8 +154,10 @@ _FOG_CACHE = _FogCache()
 
 
 class KeSSieAttentionImpl:
-    """Per-layer attention: with the fog active, decode and chunked prefill run
-    in this library's paged kernels with the fog bias applied to the scores;
+    """Per-layer attention: with the fog active, a decode step runs in the paged
+    decode and any other step (prompt chunks, drafts, decodes mixed) in one
+    ragged-chunk call, neither reading a length back to the host, with the fog
+    bias applied to the scores;
     otherwise (fog off, profiling run, features the kernels do not cover) the
     wrapped vLLM implementation runs.  Attributes and methods not defined here
     (e.g. the KV-cache write) are the wrapped implementation's."""
@@ -178,8 +180,6 @@ class KeSSieAttentionImpl:
             self._window = int(sw[0]) + 1                 # vLLM keeps (window - 1, 0)
         else:
             self._window = int(sw)
-        self._meta_ref = None
-        self._meta_host = None
 
     def __getattr__(self, name):
         return getattr(object.__getattribute__(self, "_inner"), name)
@@ -210,15 +210,6 @@ class KeSSieAttentionImpl:
                                        output_block_scale)
         return self._fog_forward(query, kv_cache, attn_metadata, output, state)
 
-    def _host_meta(self, md):
-        """Query offsets and sequence lengths on the host, once per step (the
-        same metadata object serves every layer of a step)."""
-        if self._meta_ref is not md:
-            qsl = md.query_start_loc.detach().cpu().tolist()
-            sl = md.seq_lens.detach().cpu().tolist()
-            self._meta_ref, self._meta_host = md, (qsl, sl)
-        return self._meta_host
-
     def _fog_forward(self, query, kv_cache, md, output, state):
         n = int(md.num_actual_tokens)
         Hq, D = self._num_heads, self._head_size
@@ -231,26 +222,9 @@ class KeSSieAttentionImpl:
         if int(md.max_query_len) == 1:                 # decode step: one launch for the batch
             ops.paged_fog_decode(q, key_cache, value_cache, bt[:n], sl[:n], out=out, **kw)
             return output
-        qsl, slh = self._host_meta(md)
-        B = len(slh)
-        b = 0
-        while b < B:
-            ql = qsl[b + 1] - qsl[b]
-            if ql <= 0:
-                b += 1
-                continue
-            r0 = qsl[b]
-            if ql == 1:                                  # a run of decode requests: one launch
-                e = b
-                while e < B and qsl[e + 1] - qsl[e] == 1:
-                    e += 1
-                ops.paged_fog_decode(q[r0:r0 + e - b], key_cache, value_cache, bt[b:e], sl[b:e],
-                                     out=out[r0:r0 + e - b], **kw)
-                b = e
-                continue
-            ops.paged_fog_prefill(q[r0:r0 + ql].unsqueeze(0), key_cache, value_cache, bt[b:b + 1], sl[b:b + 1],
-                                  causal=True, out=out[r0:r0 + ql].unsqueeze(0), max_kv_len=int(slh[b]), **kw)
-            b += 1
+        # a mixed step (prompt chunks, drafts, decodes): one call for the batch, lengths read on the device
+        B = sl.shape[0]
+        ops.paged_fog_chunks(q, key_cache, value_cache, bt[:B], md.query_start_loc[:B + 1], sl, out=out, **kw)
         return output
 
 

@@ -615,8 +615,8 @@ def step_tables(context_lens: torch.Tensor, query_lens: torch.Tensor, block_tabl
     if out is None:
         # one allocation for the int32 outputs
         flat = torch.empty(2 * R + 2 + num_tokens, dtype=torch.int32, device=dev)
-        res = StepTables(flat.narrow(0, 0, R + 1), flat.narrow(0, R + 1, R), flat.narrow(0, 2 * R + 2, num_tokens),
-                         torch.empty(num_tokens, dtype=torch.int64, device=dev), flat.narrow(0, 2 * R + 1, 1))
+        start, seq, used, pos = flat.split_with_sizes((R + 1, R, 1, num_tokens))
+        res = StepTables(start, seq, pos, torch.empty(num_tokens, dtype=torch.int64, device=dev), used)
     else:
         res = out
         for name, t, n, dt in zip(StepTables._fields, out, (R + 1, R, num_tokens, num_tokens, 1),

@@ -648,3 +648,43 @@ def test_step_of_all_three(captured):
         count.sub_(t.pages_used)
         ctx = t.seq_lens.clone()
     assert count.item() == P - sum(-(-int(c) // ps) for c in ctx)
+
+
+def test_attention_impl_mixed_step_is_captured_without_a_host_read():
+    """KeSSieAttentionImpl.forward of a mixed step inside a CUDA graph, replayed
+    with other lengths (the padded batch's rows behind the last token stay)."""
+    from types import SimpleNamespace
+
+    from kessie_b200 import kessie_attention as A
+    A.KESSIE_STATE.update(fog_alpha=1.5, fog_start=0.5, prompt_len=10, recall_positions=[], recall_boost=0.0)
+    A.KESSIE_STATE.enabled = True
+    try:
+        c = _Case(41, [1, 60, 7, 0], [900, 300, 77, 0], 8, 2, 128, 16, "fp16", layout="vllm", pad=4)
+        inner = SimpleNamespace(num_heads=8, num_kv_heads=2, head_size=128, scale=128 ** -0.5, sliding_window=None)
+        impl = A.KeSSieAttentionImpl(_inner_impl=inner)
+        cache = torch.stack([c.k, c.v])
+        md = SimpleNamespace(num_actual_tokens=72, max_query_len=60, query_start_loc=c.start, seq_lens=c.seq,
+                             block_table=c.bt)
+        out = torch.full((72, 8 * 128), 2.0, dtype=torch.float16, device="cuda")
+        impl.forward(None, c.q, None, None, cache, md, out)           # sets up what a first call sets up
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            impl.forward(None, c.q, None, None, cache, md, out)
+        c.start.copy_(_i32([0, 5, 6, 68, 68]))
+        c.seq.copy_(_i32([800, 250, 70, 0]))
+        c.q_lens, c.kv_lens = [5, 1, 62, 0], [800, 250, 70, 0]
+        out.fill_(2.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (out[68:] == 2.0).all()
+
+        def bias(s):                                                  # in fp16, as torch's operations round it
+            fb = int(s * 0.5)
+            j = torch.arange(s, device="cuda", dtype=torch.float64).half()
+            t = (j.float() / max(fb, 1)).half()
+            d = (1.0 - t.float()).half()
+            d = (d.float() * d.float()).half()
+            return torch.where(torch.arange(s, device="cuda") < fb, (d.float() * -1.5).half(), 0).double()
+        c.check(out.view(72, 8, 128), bias=bias)
+    finally:
+        A.KESSIE_STATE.update(prompt_len=0)
