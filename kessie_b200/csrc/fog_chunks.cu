@@ -35,8 +35,8 @@
 // row), 8 Q and K producer, 9 / 11 MMA issuers of A / B (one thread each; 9
 // owns the TMEM), 10 V producer and fog weights.  TMEM columns: S_A [0,128) S_B
 // [128,256) O_A [256,..) O_B [384,..); P (16-bit pairs) overwrites the first 64
-// columns of its S.  Per key tile a chain's issuer waits for P (in two halves, so
-// that the product starts under the second half's exponentials: 12.0 -> 11.7
+// columns of its S.  Per key tile a chain's issuer waits for P (three quarters, then
+// the rest, so that the product starts under the last exponentials: 12.1 -> 11.6
 // Mcycles at 4,096 tokens over 131k keys), issues O += P V and S = Q K^T of its
 // next key tile into the region that P leaves, so one chain's MMAs run under the
 // other's softmax.  One issuer for both chains was
@@ -516,7 +516,7 @@ __device__ __forceinline__ float softmax_p(const uint32_t (&sv)[4][32], uint32_t
             pk[i] = ptx::pack2<BF16>(p0, p1);
         }
         ptx::tmem_st16(sreg + c * 16, pk);
-        if (c == 1) {
+        if (c == 2) {
             ptx::tmem_st_wait();
             ptx::tc_fence_before();
             __syncwarp();
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
     uint64_t* o_full = p_full + 2;
     uint64_t* o_free = o_full + 2;                 // every softmax warp is done with the piece's O
     uint64_t* ml_full = o_free + 1;                // B's (m, l) of a single tile
-    uint64_t* ph_full = ml_full + 1;               // [2] first half of P
+    uint64_t* ph_full = ml_full + 1;               // [2] first three quarters of P
     Plan* plan = reinterpret_cast<Plan*>(smem + C::kPlan);
     uint32_t* slot = reinterpret_cast<uint32_t*>(smem + C::kPlan + 80);
 
@@ -747,13 +747,13 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                 ptx::tc_fence_after();
                 mma_ts(tO, tS, vlo, kv_hi, idPV, ev > 0 ? 1u : 0u);
 #pragma unroll
-                for (int kk = 1; kk < 4; ++kk) mma_ts(tO, tS + kk * 8, vlo + kk * (grp >> 3), kv_hi, idPV, 1u);
+                for (int kk = 1; kk < 6; ++kk) mma_ts(tO, tS + kk * 8, vlo + kk * (grp >> 3), kv_hi, idPV, 1u);
                 ok = ptx::mbar_wait(&p_full[x], pc & 1u);
                 ++pc;
                 if (!ok) break;
                 ptx::tc_fence_after();
 #pragma unroll
-                for (int kk = 4; kk < 8; ++kk) mma_ts(tO, tS + kk * 8, vlo + kk * (grp >> 3), kv_hi, idPV, 1u);
+                for (int kk = 6; kk < 8; ++kk) mma_ts(tO, tS + kk * 8, vlo + kk * (grp >> 3), kv_hi, idPV, 1u);
                 if (ev == nev - 1) ptx::umma_commit(&o_full[x]);
                 ptx::umma_commit(&v_empty[st]);
                 if (single) ptx::umma_commit(&v_empty[st]);
@@ -1010,10 +1010,14 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
     }
 }
 
-// Joins the pieces of cut tiles: block (c, y) takes 32 rows of the tile whose
-// second piece opens CTA c's range.  Its first piece is in the second slot of
-// the CTA before, the others in the first slots of c, c + 1, ... to the one
-// that ends the tile; they are joined in that order.
+// Joins the pieces of cut tiles: blocks (c, *) take the tile whose second piece
+// opens CTA c's range, 32 rows a block, 8 columns a warp.  The tile's first
+// piece is in the second slot of the CTA before, the others in the first slots of
+// c, c + 1, ... to the one that ends the tile; they are joined in that order, the
+// loads of kMergeBatch pieces in flight (one at a time took 32.6 us for the 19
+// pieces a tile of 17 queries over 262k keys).
+constexpr int kMergeBatch = 4;                       // pieces in flight
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) fog_chunks_merge_kernel(const ChunkParams p, int ctas) {
     ptx::grid_dependency_wait();
@@ -1024,47 +1028,70 @@ __global__ void __launch_bounds__(256) fog_chunks_merge_kernel(const ChunkParams
     int before = c - 1;                                          // the CTA with the piece before this one
     while (before > 0 && desc[before].state == kNoPiece) --before;
     if (desc[before].state == kMidTile && !desc[before].ends) return;      // an earlier boundary cut this tile
-    __shared__ int piece[kThreads];                              // the tile's pieces in order: slots
+    __shared__ int piece[kThreads + 1];                          // the tile's pieces in order: slots
     __shared__ int count;
-    if (threadIdx.x == 0) {
-        int n = 0;
-        piece[n++] = 2 * before + 1;
-        piece[n++] = 2 * c;
-        for (int e = d.ends, k = c + 1; !e && k < ctas; ++k)
-            if (desc[k].state == kMidTile) { piece[n++] = 2 * k; e = desc[k].ends; }
-        count = n;
+    if (threadIdx.x < 32) {
+        // a warp looks at 32 CTAs at a time, up to the piece that ends the tile
+        const int lane = threadIdx.x;
+        int n = 2;
+        if (lane == 0) { piece[0] = 2 * before + 1; piece[1] = 2 * c; }
+        for (int k0 = c + 1, over = d.ends; !over && k0 < ctas; k0 += 32) {
+            const bool in = k0 + lane < ctas;
+            const bool mid = in && desc[k0 + lane].state == kMidTile;
+            const unsigned mids = __ballot_sync(0xffffffffu, mid), ends = __ballot_sync(0xffffffffu, mid && desc[k0 + lane].ends);
+            const unsigned upto = ends ? (ends & -ends) * 2 - 1 : 0xffffffffu;          // lanes to the end of the tile
+            const unsigned mine = mids & upto;
+            if ((mine >> lane) & 1u) piece[n + __popc(mine & ((1u << lane) - 1))] = 2 * (k0 + lane);
+            n += __popc(mine);
+            over = ends != 0;
+        }
+        if (lane == 0) count = n;
     }
     __syncthreads();
-    const int n = count - 1;
-    const int rows = d.ntok <= p.TH ? d.ntok * p.G : p.TH * p.G + 128;
+    const int n = count;
     const char* slots = p.ws + (size_t)ctas * sizeof(PieceDesc);
-    auto slot = [&](int i) { return slots + (size_t)piece[i] * Cfg<D>::kSlotBytes; };
-    const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;   // a warp: 32 rows, 8 columns at a time
-    const int row = blockIdx.y * 32 + lane;
-    const int half = row >> 7, r = row & 127;
-    const int tok = half * p.TH + r / p.G;
-    if (row >= rows || r >= p.TH * p.G || tok >= d.ntok) return;
-    float m = -INFINITY;
-    for (int i = 0; i <= n; ++i) m = fmaxf(m, reinterpret_cast<const float2*>(slot(i) + (size_t)256 * D * 4)[row].x);
-    uint16_t* o = static_cast<uint16_t*>(p.o) + (int64_t)(d.row0 + tok) * p.o_st + (int64_t)(d.hk * p.G + r % p.G) * p.o_sh;
-    for (int c8 = grp; c8 < D / 8; c8 += 8) {
-        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
-        for (int i = 0; i <= n; ++i) {
-            const char* s = slot(i);
-            const float2 ml = reinterpret_cast<const float2*>(s + (size_t)256 * D * 4)[row];
-            const float f = ml.x == -INFINITY ? 0.f : ptx::ex2(ml.x - m);
-            const float4 a = reinterpret_cast<const float4*>(s)[(2 * c8) * 256 + row];
-            const float4 b = reinterpret_cast<const float4*>(s)[(2 * c8 + 1) * 256 + row];
-            l += ml.y * f;
-            acc[0] += a.x * f; acc[1] += a.y * f; acc[2] += a.z * f; acc[3] += a.w * f;
-            acc[4] += b.x * f; acc[5] += b.y * f; acc[6] += b.z * f; acc[7] += b.w * f;
-        }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        uint32_t pk[4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = blockIdx.y * 32 + lane, half = row >> 7, r = row & 127, tok = half * p.TH + r / p.G;
+    const int c8 = blockIdx.z * 8 + warp;
+    if (r >= p.TH * p.G || tok >= d.ntok || (half && d.ntok <= p.TH)) return;
+    // running maximum over batches of pieces
+    float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < n; i0 += kMergeBatch) {
+        float2 ml[kMergeBatch];
+        float4 x[kMergeBatch][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pk[i] = ptx::pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-        *reinterpret_cast<uint4*>(o + c8 * 8) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+        for (int u = 0; u < kMergeBatch; ++u) {
+            const char* s = slots + (size_t)piece[min(i0 + u, n - 1)] * Cfg<D>::kSlotBytes;
+            ml[u] = reinterpret_cast<const float2*>(s + (size_t)256 * D * 4)[row];
+            x[u][0] = reinterpret_cast<const float4*>(s)[(2 * c8) * 256 + row];
+            x[u][1] = reinterpret_cast<const float4*>(s)[(2 * c8 + 1) * 256 + row];
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < kMergeBatch; ++u) {
+            if (i0 + u >= n) ml[u].x = -INFINITY;
+            top = fmaxf(top, ml[u].x);
+        }
+        const float old = m == -INFINITY ? 0.f : ptx::ex2(m - top);
+        l *= old;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] *= old;
+#pragma unroll
+        for (int u = 0; u < kMergeBatch; ++u) {
+            const float f = ml[u].x == -INFINITY ? 0.f : ptx::ex2(ml[u].x - top);
+            l += ml[u].y * f;
+            const float* v = &x[u][0].x;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] += f == 0.f ? 0.f : v[i] * f;
+        }
+        m = top;
     }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint32_t pk[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pk[i] = ptx::pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    uint16_t* o = static_cast<uint16_t*>(p.o) + (int64_t)(d.row0 + tok) * p.o_st + (int64_t)(d.hk * p.G + r % p.G) * p.o_sh;
+    *reinterpret_cast<uint4*>(o + c8 * 8) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
 }
 
 // Tensor map of K (or V); fills the box geometry of `p`.  The 8-row groups of
@@ -1134,7 +1161,7 @@ int launch_chunks(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap&
     LaunchOrderGuard order;
     claim_early_reads(st, nullptr, 0, wrote, 2);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid - 1, 8);
+    cfg.gridDim = dim3(grid - 1, 8, D / 64);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
