@@ -72,8 +72,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kProducerRegs = 88;
 static_assert(256 * kSoftmaxRegs + 128 * kProducerRegs <= kThreads * kLaunchRegs, "register split exceeds the pool");
 
-// Plan weights of a 128-key tile (pair / single) and of starting and ending a tile.
-constexpr int kCostPair = 3, kCostSingle = 2, kCostTile = 4;
+// Plan weights of a 128-key tile (pair / single) and of starting and ending a tile
+// (with 4 for the latter, 208 short sequences took 209 us, with 7 188 us, with 14
+// 193 us; an 8,192-token prompt 530, 498, 506 us).
+constexpr int kCostPair = 3, kCostSingle = 2, kCostTile = 7;
 
 // Whole tiles in waves first when the mean tile costs at least this (8k keys; at 2,048 tokens over 65k keys the pure
 // cut read 6.2 GB for 0.27 GB of K/V), at most kMaxWhole a CTA.
