@@ -12,6 +12,7 @@ strides so both the KeSSie layout [P, ps, 2, H, D]
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import threading
 from typing import NamedTuple, Optional, Sequence, Tuple
@@ -62,9 +63,9 @@ def _need_cuda(*ts):
 def _i32(t: Optional[torch.Tensor], device) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if not torch.is_tensor(t):
+    if not isinstance(t, torch.Tensor):
         t = torch.as_tensor(t, dtype=torch.int32, device=device)
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         t = t.to(torch.int32)
     return t.contiguous()
 
@@ -88,14 +89,17 @@ def _stream_workspace(nbytes: int, dev: torch.device, tag: str, handle: int) -> 
     so calls on two streams never share one; a capture gets a buffer of its
     graph's memory pool, so two captured graphs may run at once.  `dev` is the
     current device."""
-    current = _stream(None, dev.index)
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
-    if handle == current:
-        return workspace(nbytes, dev, f"{tag}@{handle}")
-    # allocated under the stream that uses it: the allocator hands memory out in that stream's order
-    with torch.cuda.stream(torch.cuda.ExternalStream(handle, device=dev)):
-        return workspace(nbytes, dev, f"{tag}@{handle}")
+    key = (dev.index, tag, handle)
+    buf = _ws_cache.get(key)
+    if buf is None or buf.numel() < nbytes:
+        with _ws_lock:
+            # allocated under the stream that uses it: the allocator hands memory out in that stream's order
+            with torch.cuda.stream(torch.cuda.ExternalStream(handle, device=dev)):
+                buf = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
+            _ws_cache[key] = buf
+    return buf
 
 
 def read_device_status(stream=None) -> int:
@@ -644,11 +648,15 @@ def _axis_positions(name: str, positions, axes: int, tokens: int, device) -> tor
     return t if tokens <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
-def _sections(name: str, sections: Sequence[int]):
-    n = len(sections)
-    if n == 0:
-        raise ValueError(f"{name}: sections must give each axis its number of frequencies")
-    return (ctypes.c_int * n)(*sections), n
+@functools.lru_cache(maxsize=64)
+def _section_array(sections: Tuple[int, ...]):
+    if not sections:
+        raise ValueError("sections must give each axis its number of frequencies")
+    return (ctypes.c_int * len(sections))(*sections), len(sections)
+
+
+def _sections(sections: Sequence[int]):
+    return _section_array(tuple(sections))
 
 
 def _rows(name: str, x: torch.Tensor):
@@ -678,7 +686,7 @@ def rope_axes_remap(k: torch.Tensor, orig_positions, target_positions, sections:
         raise ValueError("rope_axes_remap: out must match k's shape and dtype")
     T, H, D = k.shape
     ks, os_ = _rows("rope_axes_remap", k), _rows("rope_axes_remap", out)
-    sec, axes = _sections("rope_axes_remap", sections)
+    sec, axes = _sections(sections)
     tgt = _axis_positions("rope_axes_remap", target_positions, axes, T, k.device)
     org = None if orig_positions is None else _axis_positions("rope_axes_remap", orig_positions, axes, T, k.device)
     _lib.check(_lib.load().kessie_rope_axes_remap_v2(
@@ -707,17 +715,19 @@ def rope_axes_insert(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, position
     T, Hq, D = q.shape
     ps_, ts_, kvs_, hs_, P, ps, Hkv, Dc = kv_layout_strides(kv, layout)
     rows = (T, Hkv, D)
-    if k.shape != rows or v.shape != rows or Dc != D or out_q.shape != q.shape:
+    if k.shape != rows or v.shape != rows or Dc != D or (out_q is not q and out_q.shape != q.shape):
         raise ValueError(f"rope_axes_insert: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, "
                          f"out_q {tuple(out_q.shape)} do not match a cache of {Hkv} heads of {Dc}")
-    if not (q.dtype == k.dtype == v.dtype == kv.dtype == out_q.dtype):
+    dt = q.dtype
+    if not (k.dtype is dt and v.dtype is dt and kv.dtype is dt and out_q.dtype is dt):
         raise TypeError("rope_axes_insert: q, k, v, out_q and the cache share one dtype")
     if kv.stride(-1) != 1:
         raise ValueError("rope_axes_insert: the cache's head_dim must be contiguous")
     if slot_mapping.numel() != T:
         raise ValueError("rope_axes_insert: slot_mapping has one entry per token")
-    qs, ks, vs, os_ = (_rows("rope_axes_insert", x) for x in (q, k, v, out_q))
-    sec, axes = _sections("rope_axes_insert", sections)
+    qs, ks = _rows("rope_axes_insert", q), _rows("rope_axes_insert", k)
+    vs, os_ = _rows("rope_axes_insert", v), _rows("rope_axes_insert", out_q)
+    sec, axes = _sections(sections)
     pos = _axis_positions("rope_axes_insert", positions, axes, T, q.device)
     slots = slot_mapping if slot_mapping.dtype == torch.int64 else slot_mapping.to(torch.int64)
     slots = slots.contiguous()
@@ -758,7 +768,7 @@ def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     ks, qs = k_cache.stride(), q.stride()
     if Dk != D or v_cache.shape != k_cache.shape or v_cache.stride() != ks:
         raise ValueError("k_cache/v_cache must be matching [P, ps, Hkv, D] views")
-    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    if k_cache.dtype is not q.dtype or v_cache.dtype is not q.dtype:
         raise TypeError("q and the cache must share a dtype")
     if ks[3] != 1:
         raise ValueError("head_dim must be contiguous")
@@ -776,10 +786,11 @@ def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     bt = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
     if bt.stride(1) != 1:
         bt = bt.contiguous()
-    qsl, sl = _i32(query_start_loc, dev), _i32(seq_lens, dev)
-    cs = _i32(clear_start, dev)
-    if cs is not None and (cs.numel() != B or cs.get_device() != index):
-        raise ValueError("paged_fog_chunks: clear_start has one entry per sequence, on q's device")
+    qsl, sl, cs = _i32(query_start_loc, dev), _i32(seq_lens, dev), None
+    if clear_start is not None:
+        cs = _i32(clear_start, dev)
+        if cs.numel() != B or cs.get_device() != index:
+            raise ValueError("paged_fog_chunks: clear_start has one entry per sequence, on q's device")
     cap = width * ps
     if max_seq_len is None:
         max_seq_len = cap
@@ -790,7 +801,7 @@ def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     lib = _lib.load()
     handle = _stream(stream, index)
     if ws is None:
-        ws = _stream_workspace(lib.kessie_paged_fog_chunks_workspace_size(Hq, Hkv, D), dev, "chunks", handle)
+        ws = _stream_workspace(_chunks_bytes(index, Hq, Hkv, D), dev, "chunks", handle)
     os_ = out.stride()
     _lib.check(lib.kessie_paged_fog_chunks_v2(
         q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], P, ps, bt.data_ptr(),
@@ -799,6 +810,11 @@ def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         None if bias is None else ctypes.byref(bias.c_struct()), out.data_ptr(), os_[0], os_[1], ws.data_ptr(),
         ws.numel(), handle), "paged_fog_chunks")
     return out
+
+
+@functools.lru_cache(maxsize=None)
+def _chunks_bytes(device_index: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    return chunks_workspace_bytes(num_q_heads, num_kv_heads, head_dim)
 
 
 def chunks_workspace_bytes(num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
