@@ -756,9 +756,10 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                 ptx::tc_fence_after();
 #pragma unroll
                 for (int kk = 6; kk < 8; ++kk) mma_ts(tO, tS + kk * 8, vlo + kk * (grp >> 3), kv_hi, idPV, 1u);
-                if (ev == nev - 1) ptx::umma_commit(&o_full[x]);
                 ptx::umma_commit(&v_empty[st]);
                 if (single) ptx::umma_commit(&v_empty[st]);
+                // last: who sees it has seen every arrival of this thread's MMAs, so none is under way when the CTA ends
+                if (ev == nev - 1) ptx::umma_commit(&o_full[x]);
                 if (ev + 1 < nev) issue_s(ev + 1);
             }
             if (nev == 0 && ok) {                                    // a single tile's only key tile is chain A's
@@ -1152,6 +1153,9 @@ int launch_chunks(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap&
             return check_launch("paged_fog_chunks: set smem attribute");
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
+    // held over both launches: a call of another host thread on this stream must not come between them (the
+    // workspace), nor a programmatic one
+    LaunchOrderGuard order;
     kern<<<grid, kThreads, Cfg<D>::kAlloc, st>>>(q, k, v, p);
     const int rc = check_launch("paged_fog_chunks");
     if (rc || grid < 2) return rc;
@@ -1160,7 +1164,6 @@ int launch_chunks(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap&
     // nothing early itself, and is on record for a programmatic launch behind it.
     const ByteRange wrote[2] = {byte_span(p.o, 2 * ((int64_t)(p.T - 1) * p.o_st + (int64_t)(p.Hkv * p.G - 1) * p.o_sh + D)),
                                 byte_span(p.ws, (int64_t)chunks_workspace_bytes(D))};
-    LaunchOrderGuard order;
     claim_early_reads(st, nullptr, 0, wrote, 2);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid - 1, 8, D / 64);

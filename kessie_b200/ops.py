@@ -85,19 +85,20 @@ def workspace(nbytes: int, device, tag: str = "default") -> torch.Tensor:
 
 
 def _stream_workspace(nbytes: int, dev: torch.device, tag: str, handle: int) -> torch.Tensor:
-    """Scratch for a call on stream `handle` of `dev`: one buffer per stream,
-    so calls on two streams never share one; a capture gets a buffer of its
-    graph's memory pool, so two captured graphs may run at once.  `dev` is the
-    current device."""
+    """Scratch for a call on stream `handle` of `dev` (the current device): one
+    buffer per stream, so calls on two streams never share one; a capture gets
+    a buffer of its graph's memory pool, so two captured graphs may run at once."""
+    if handle != _stream(None, dev.index):
+        # allocated under the stream that uses it: the allocator hands memory out in that stream's order
+        with torch.cuda.stream(torch.cuda.ExternalStream(handle, device=dev)):
+            return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
     key = (dev.index, tag, handle)
     buf = _ws_cache.get(key)
     if buf is None or buf.numel() < nbytes:
+        buf = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
         with _ws_lock:
-            # allocated under the stream that uses it: the allocator hands memory out in that stream's order
-            with torch.cuda.stream(torch.cuda.ExternalStream(handle, device=dev)):
-                buf = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
             _ws_cache[key] = buf
     return buf
 
@@ -775,7 +776,7 @@ def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     B, width = block_table.shape
     if query_start_loc.numel() != B + 1 or seq_lens.numel() != B:
         raise ValueError("paged_fog_chunks: block_table [B, maxP], query_start_loc [B + 1], seq_lens [B]")
-    if qs[2] != 1 or (qs[0] | qs[1]) % 8 or q.data_ptr() % 16:
+    if qs[2] != 1 or (qs[0] | qs[1]) % 8 or qs[0] <= 0 or qs[1] <= 0 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)      # rows the kernel cannot load: a copy
         qs = q.stride()
     if out is None:
@@ -791,6 +792,8 @@ def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         cs = _i32(clear_start, dev)
         if cs.numel() != B or cs.get_device() != index:
             raise ValueError("paged_fog_chunks: clear_start has one entry per sequence, on q's device")
+    if bias is not None and bias.bits is not None and bias.bits.get_device() != index:
+        raise ValueError("paged_fog_chunks: the bias's recalled positions are on another device")
     cap = width * ps
     if max_seq_len is None:
         max_seq_len = cap

@@ -128,6 +128,16 @@ def test_step_tables_free_count_int64_lengths_and_reused_outputs():
     assert count.item() == len(free) and b.pages_used.item() == want[4]
 
 
+def test_step_tables_without_requests_or_tokens():
+    from kessie_b200 import ops
+    none = _i32([])
+    got = ops.step_tables(none, none, torch.empty(0, 4, dtype=torch.int32, device="cuda"), 16, _i32([1, 2]), 3)
+    assert got.query_start_loc.tolist() == [0] and got.slot_mapping.tolist() == [-1] * 3 and got.pages_used.item() == 0
+    table = torch.full((1, 4), -1, dtype=torch.int32, device="cuda")
+    got = ops.step_tables(_i32([3]), _i32([0]), table, 16, none, 0)          # no new token, no free page
+    assert got.query_start_loc.tolist() == [0, 0] and got.seq_lens.tolist() == [3] and (table == -1).all()
+
+
 def test_step_tables_far_slots_pass_32_bits():
     from kessie_b200 import ops
     table = torch.tensor([[200_000_000, -1]], dtype=torch.int32, device="cuda")
@@ -580,6 +590,42 @@ def test_chunks_two_captured_graphs_replayed_at_once():
     torch.cuda.synchronize()
     a.kv_lens = [500, 8, 20000]
     a.check(oa)
+
+
+def test_chunks_from_two_host_threads_on_one_stream():
+    """The kernel and its merge stay together, whoever else launches there."""
+    import threading
+    stream = torch.cuda.Stream()
+    cases = [_Case(25, [1, 7, 33], [30000, 9000, 20000], 8, 1, 128, 16, "bf16"),
+             _Case(26, [16, 1], [25000, 12000], 8, 1, 128, 16, "bf16")]
+    want = [c.run() for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(stream):
+            for _ in range(40):
+                got[i].append(cases[i].run())
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+
+
+def test_chunks_broadcast_queries_empty_batch_and_workspace():
+    from kessie_b200 import ops
+    c = _Case(27, [3, 2], [300, 200], 8, 2, 64, 16, "bf16")
+    c.q = c.q[:1].expand(5, 8, 64)                                    # one query row for all tokens (stride 0)
+    c.check(c.run())
+    ws = torch.empty(ops.chunks_workspace_bytes(8, 2, 64), dtype=torch.uint8, device="cuda").fill_(255)
+    assert torch.equal(c.run(ws=ws), c.run())                         # leftover contents are never read
+    with pytest.raises(Exception, match="workspace"):
+        c.run(ws=ws[:-16])
+    empty = ops.paged_fog_chunks(c.q[:0], c.k, c.v, c.bt, c.start, c.seq)
+    assert empty.shape == (0, 8, 64)
+    with pytest.raises(Exception, match="not both"):
+        c.run(clear_start=_i32([5, 5]), bias=ops.FogBias(1.0, 0.5, dtype=torch.float32))
 
 
 # ------------------------------------------------------------------ a step of all three
