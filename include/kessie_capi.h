@@ -575,7 +575,8 @@ int kessie_paged_fog_decode_cp_v2(const void* q, int64_t q_stride_b, int64_t q_s
  *   tokens in request order; slot = page * page_size + position % page_size;
  *   rows past the last token (a padded batch) get position 0 and slot -1;
  *   pages_used int32 [1]: entries taken from free_pages (free_pages itself
- *   and free_count are not changed).
+ *   and free_count are not changed).  No output may share memory with an
+ *   input.
  * KESSIE_DEV_BAD_ARG is recorded for a negative length (taken as 0), a
  * sequence past the table's width, more tokens than num_tokens, or more pages
  * than are free (table entries -1); KESSIE_DEV_BAD_PAGE_ID for a page id
@@ -631,9 +632,10 @@ int kessie_rope_axes_insert_v2(const void* q, int64_t q_token_stride, int64_t q_
  * 128, rows 16-byte aligned); rows query_start_loc[b] .. query_start_loc[b+1)
  * (int32 [batch + 1]) belong to sequence b, the last of them at position
  * seq_lens[b] - 1 (batch <= 8192).  Keys j < min(seq_lens[b], max_seq_len) of
- * block_table[b] (max_seq_len within the table's rows) are seen when j <= position (is_causal or a window) and
- * position - j < window_size (window_size > 0); is_causal 0 without a window
- * attends to all keys of another sequence (cross attention).
+ * block_table[b] (max_seq_len within the table's rows) are seen when j <=
+ * position (is_causal or a window) and position - j < window_size
+ * (window_size > 0); is_causal 0 without a window attends to all keys of
+ * another sequence (cross attention).
  * Fog: clear_start / fog_alpha as in the decode (on V), or bias (added to the
  * scaled scores, by key position, kv_len = the sequence's keys); both nullable,
  * not both at once.
@@ -642,7 +644,8 @@ int kessie_rope_axes_insert_v2(const void* q, int64_t q_token_stride, int64_t q_
  * pages may hold anything; keys that some of its rows see must be finite.
  * A page id outside [0, num_pages) reads as zero keys and values and records
  * KESSIE_DEV_BAD_PAGE_ID; a length past max_seq_len, or offsets that leave
- * [0, num_tokens] or fall, are cut and record KESSIE_DEV_BAD_ARG.
+ * [0, num_tokens], are cut and record KESSIE_DEV_BAD_ARG; offsets that fall
+ * record it too, and nothing is computed.  out may be q itself.
  * workspace: kessie_paged_fog_chunks_workspace_size() bytes, 16-byte aligned,
  * no initialisation; calls that can overlap need one each. */
 size_t kessie_paged_fog_chunks_workspace_size(int num_q_heads, int num_kv_heads, int head_dim);

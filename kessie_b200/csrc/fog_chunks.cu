@@ -25,11 +25,11 @@
 // lengths.  Cutting puts the CTAs at different keys of a head at any time, so
 // each would fetch its K/V for itself: when several tiles share a long context
 // (kWholeCost), the CTAs first take whole tiles in waves -- neighbours run
-// through the same keys together, from L2 -- and cut only what is left
-// (1,024-token chunk: see kWholeCost).  Every CTA derives the plan itself from
-// the length arrays.  A tile cut by a range boundary leaves fp32 partials (O, m, l) of each piece in the
-// workspace, at most two a CTA, and fog_chunks_merge_kernel joins them in
-// order, so results do not depend on timing.
+// through the same keys together, from L2 -- and cut only what is left.
+// Every CTA derives the plan itself from the length arrays.  A tile cut by a
+// range boundary leaves fp32 partials (O, m, l) of each piece in the workspace,
+// at most two a CTA, and fog_chunks_merge_kernel joins them in order, so
+// results do not depend on timing.
 //
 // CTA = 12 warps: 0-3 / 4-7 softmax of A / B (one row per thread: TMEM lane =
 // row), 8 Q and K producer, 9 / 11 MMA issuers of A / B (one thread each; 9
@@ -46,6 +46,12 @@
 // K/V come straight from the pages: one TMA box per page (up to 128 tokens)
 // lands as [token / 8][D / 64][8][64] with 128-byte swizzle, whose 8-row groups
 // have one stride, so a K or V tile of any page size is one matrix operand.
+//
+// Bound by: the serial chain scores -> exponentials -> P -> product of chunks
+// (tensor pipe 60 %, MUFU 61 % busy; 4,096 tokens of 32 / 8 heads of 128 over
+// 131,072 keys, bf16: 6.9 ms = 1,250 TFLOP/s, 9.2 ms with the V fog, where the
+// power cap holds the clock near 1.75 GHz), HBM for decodes (28 of 1k-16k keys:
+// 6.0 TB/s, every key read once), launches and the plan for the smallest (17 us).
 //
 // Every mbarrier wait is bounded; on a timeout all warps still reach the final
 // barrier and the TMEM is freed.
@@ -288,12 +294,15 @@ __device__ __forceinline__ void make_plan(const ChunkParams& p, int64_t* pre, in
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t ctas = gridDim.x;
     int64_t W = 0, tiles = 0;
-    bool bad = false;
+    bool bad = false, unordered = false;
     const int TT = 2 * p.TH;
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
         const int b = b0 + tid;
         Seq s{0, 0, 0, 0};
-        if (b < p.B) s = load_seq(p, b, &bad);
+        if (b < p.B) {
+            s = load_seq(p, b, &bad);
+            unordered |= __ldg(p.start + b + 1) < __ldg(p.start + b);
+        }
         const int nt = (s.n + TT - 1) / TT;
         int64_t c = 0;
         if (nt <= 2)
@@ -326,7 +335,8 @@ __device__ __forceinline__ void make_plan(const ChunkParams& p, int64_t* pre, in
     }
     if (bad && blockIdx.x == 0) record_status(p.status, KESSIE_DEV_BAD_ARG);
     W *= p.Hkv;                                    // pre stays per head
-    __syncthreads();
+    // starts that fall would let sequences share rows, without a bound on the tiles: nothing is computed
+    if (__syncthreads_or(unordered)) W = tiles = 0;
     // whole tiles first, where several share a long context
     const int64_t n_tiles = tiles * p.Hkv;
     int whole = 0;
@@ -1228,6 +1238,8 @@ extern "C" int kessie_paged_fog_chunks_v2(const void* q, int64_t q_stride_t, int
         ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(k_cache) |
           reinterpret_cast<uintptr_t>(v_cache)) & 15))
         return set_error(KESSIE_ERR_ARG, "paged_fog_chunks_v2: q, out and cache rows must be 16-byte aligned");
+    if ((num_tokens > 1 && o_stride_t == 0) || (num_q_heads > 1 && o_stride_h == 0))
+        return set_error(KESSIE_ERR_ARG, "paged_fog_chunks_v2: rows of out share memory");
     const size_t need = kessie_paged_fog_chunks_workspace_size(num_q_heads, num_kv_heads, head_dim);
     if (!workspace || workspace_bytes < need)
         return set_error(KESSIE_ERR_WORKSPACE, "paged_fog_chunks_v2: workspace %zu < %zu", workspace_bytes, need);
@@ -1241,10 +1253,12 @@ extern "C" int kessie_paged_fog_chunks_v2(const void* q, int64_t q_stride_t, int
     p.table = block_table; p.table_stride = block_table_stride;
     p.start = query_start_loc; p.seq = seq_lens;
     p.clear_start = fog_alpha > 0.f ? clear_start : nullptr; p.fog_alpha = fog_alpha;
-    p.window = window_size > 0 ? window_size : 0; p.causal = is_causal ? 1 : 0;
+    // a window as wide as the longest sequence masks no more than causality does
+    const bool wide = window_size > 0 && window_size >= max_seq_len;
+    p.window = window_size > 0 && !wide ? window_size : 0; p.causal = is_causal || wide ? 1 : 0;
     p.scale_log2 = sm_scale * kLog2e;
     p.B = batch; p.T = num_tokens; p.Hkv = num_kv_heads; p.G = num_q_heads / num_kv_heads; p.TH = 128 / p.G;
-    p.max_seq = max_seq_len;
+    p.max_seq = max_seq_len < INT_MAX - 255 ? max_seq_len : INT_MAX - 255;     // key tiles end below 2^31
     const int brc = fog_bias_from_c(bias, &p.bias);
     if (brc) return brc;
     if (p.bias.on && p.clear_start)

@@ -22,9 +22,9 @@
 // token's angles are computed once over its threads, stay in registers, and
 // nothing is shared.  Forms that shared angles through shared memory (a warp or
 // a CTA per block of tokens) issued 500 to 570 instructions a token for the remap
-// of 65,536 keys of 8 fp16 heads and took 55 to 76 us; this one takes 45.3 us,
-// 230 instructions a token (5.96 TB/s; a plain copy of the same bytes: 44 us).
-// 8,197 new tokens of 32 + 8 + 8 bf16 heads into their slots: 38 us, 5.3 TB/s.
+// of 65,536 keys of 8 fp16 heads and took 55 to 76 us; this one takes 46.6 us,
+// 246 instructions a token (5.8 TB/s; a plain copy of the same bytes: 44 us).
+// 8,197 new tokens of 32 + 8 + 8 bf16 heads into their slots: 38.7 us, 5.2 TB/s.
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -362,6 +362,8 @@ int run_rope_axes(RopeAxesParams& p, int dtype, const int* sections, int interle
     const RopeAxesTable& tab = last.tab;
     p.half = last.half;
     if (2 * p.half > p.D) return set_error(KESSIE_ERR_ARG, "rope_axes: %d rotated dimensions of %d", 2 * p.half, p.D);
+    if ((p.T > 1 && p.Hq && p.oq_st == 0) || (p.Hq > 1 && p.oq_sh == 0))
+        return set_error(KESSIE_ERR_ARG, "rope_axes: rows of the output share memory");
     p.status = device_status_ptr();
     if (p.T == 0) { clear_error(); return KESSIE_OK; }
     switch (dtype) {

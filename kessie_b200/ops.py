@@ -85,13 +85,10 @@ def workspace(nbytes: int, device, tag: str = "default") -> torch.Tensor:
 
 
 def _stream_workspace(nbytes: int, dev: torch.device, tag: str, handle: int) -> torch.Tensor:
-    """Scratch for a call on stream `handle` of `dev` (the current device): one
-    buffer per stream, so calls on two streams never share one; a capture gets
-    a buffer of its graph's memory pool, so two captured graphs may run at once."""
-    if handle != _stream(None, dev.index):
-        # allocated under the stream that uses it: the allocator hands memory out in that stream's order
-        with torch.cuda.stream(torch.cuda.ExternalStream(handle, device=dev)):
-            return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
+    """Scratch for a call on the current stream (`handle`) of `dev` (the current
+    device): one buffer per stream, so calls on two streams never share one; a
+    capture gets a buffer of its graph's memory pool, so two captured graphs may
+    run at once."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
     key = (dev.index, tag, handle)
@@ -581,6 +578,19 @@ def _one_device(name: str, *ts) -> int:
     return index
 
 
+def _elsewhere(index: int, stream):
+    """(context, stream) of a call that is not on the current device and
+    stream, else None: its conversions and allocations are made under the
+    device and the stream that use them, in that stream's order."""
+    if index != torch.cuda.current_device():
+        return torch.cuda.device(index), stream
+    if stream is not None:
+        handle = _stream(stream)
+        if handle != _stream(None, index):
+            return torch.cuda.stream(torch.cuda.ExternalStream(handle, device=torch.device("cuda", index))), None
+    return None
+
+
 def step_tables(context_lens: torch.Tensor, query_lens: torch.Tensor, block_table: torch.Tensor, page_size: int,
                 free_pages: torch.Tensor, num_tokens: int, num_pages: Optional[int] = None,
                 free_count: Optional[torch.Tensor] = None, out: Optional["StepTables"] = None,
@@ -596,14 +606,17 @@ def step_tables(context_lens: torch.Tensor, query_lens: torch.Tensor, block_tabl
     written into block_table.  num_tokens is the size of the per-token outputs
     (the batch's new tokens, or the padded size of a captured batch: rows past
     the last token get position 0 and slot -1).  num_pages (the pool's size)
-    bounds the page ids.  `out` reuses an earlier result's tensors.  Lengths
+    bounds the page ids.  `out` reuses an earlier result's tensors, none of them
+    one of this call's inputs.  Lengths
     that do not fit are cut and recorded in the device status
     (read_device_status), with -1 for the pages and slots concerned."""
     index = _one_device("step_tables", block_table, context_lens, query_lens, free_pages, free_count, *(out or ()))
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return step_tables(context_lens, query_lens, block_table, page_size, free_pages, num_tokens, num_pages,
-                               free_count, out, stream)
+    if index != torch.cuda.current_device() or stream is not None:
+        away = _elsewhere(index, stream)
+        if away:
+            with away[0]:
+                return step_tables(context_lens, query_lens, block_table, page_size, free_pages, num_tokens, num_pages,
+                                   free_count, out, away[1])
     dev = block_table.device
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
             (block_table.shape[1] > 1 and block_table.stride(1) != 1):
@@ -680,9 +693,12 @@ def rope_axes_remap(k: torch.Tensor, orig_positions, target_positions, sections:
     exact to fp32 at any int32 position."""
     out = k if out is None else out
     index = _one_device("rope_axes_remap", k, out)
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return rope_axes_remap(k, orig_positions, target_positions, sections, rope_theta, interleaved, out, stream)
+    if index != torch.cuda.current_device() or stream is not None:
+        away = _elsewhere(index, stream)
+        if away:
+            with away[0]:
+                return rope_axes_remap(k, orig_positions, target_positions, sections, rope_theta, interleaved, out,
+                                       away[1])
     if out.shape != k.shape or out.dtype != k.dtype:
         raise ValueError("rope_axes_remap: out must match k's shape and dtype")
     T, H, D = k.shape
@@ -709,10 +725,12 @@ def rope_axes_insert(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, position
     rope_axes_remap; slots must be distinct.  One launch."""
     out_q = q if out_q is None else out_q
     index = _one_device("rope_axes_insert", q, k, v, kv, slot_mapping, out_q)
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return rope_axes_insert(q, k, v, positions, sections, kv, slot_mapping, rope_theta, interleaved, out_q,
-                                    layout, stream)
+    if index != torch.cuda.current_device() or stream is not None:
+        away = _elsewhere(index, stream)
+        if away:
+            with away[0]:
+                return rope_axes_insert(q, k, v, positions, sections, kv, slot_mapping, rope_theta, interleaved,
+                                        out_q, layout, away[1])
     T, Hq, D = q.shape
     ps_, ts_, kvs_, hs_, P, ps, Hkv, Dc = kv_layout_strides(kv, layout)
     rows = (T, Hkv, D)
@@ -756,14 +774,17 @@ def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     views, block_table [B, maxP].  causal=False without a window attends to
     all of the sequence's keys, whatever the number of queries (cross
     attention).  clear_start / fog_alpha or bias as in paged_fog_decode.
-    Returns out [T, Hq, D]; rows that see no key are 0, rows of no sequence (a
-    padded batch) are not written.  Scratch memory: one buffer per stream, a
+    Returns out [T, Hq, D] (which may be q itself); rows that see no key are 0,
+    rows of no sequence (a padded batch) are not written, and none when
+    query_start_loc falls.  Scratch memory: one buffer per stream, a
     graph capture gets its own; or `ws` (chunks_workspace_bytes() bytes)."""
     index = _one_device("paged_fog_chunks", q, k_cache, v_cache, block_table, query_start_loc, seq_lens, out, ws)
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return paged_fog_chunks(q, k_cache, v_cache, block_table, query_start_loc, seq_lens, clear_start, fog_alpha,
-                                    window_size, causal, sm_scale, max_seq_len, out, stream, ws, bias)
+    if index != torch.cuda.current_device() or stream is not None:
+        away = _elsewhere(index, stream)
+        if away:
+            with away[0]:
+                return paged_fog_chunks(q, k_cache, v_cache, block_table, query_start_loc, seq_lens, clear_start,
+                                        fog_alpha, window_size, causal, sm_scale, max_seq_len, out, away[1], ws, bias)
     T, Hq, D = q.shape
     P, ps, Hkv, Dk = k_cache.shape
     ks, qs = k_cache.stride(), q.stride()
@@ -796,7 +817,7 @@ def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError("paged_fog_chunks: the bias's recalled positions are on another device")
     cap = width * ps
     if max_seq_len is None:
-        max_seq_len = cap
+        max_seq_len = min(cap, 2 ** 31 - 1)
     elif max_seq_len > cap:
         raise ValueError(f"max_seq_len {max_seq_len} exceeds the block table capacity {cap}")
     if sm_scale is None:

@@ -628,6 +628,62 @@ def test_chunks_broadcast_queries_empty_batch_and_workspace():
         c.run(clear_start=_i32([5, 5]), bias=ops.FogBias(1.0, 0.5, dtype=torch.float32))
 
 
+def test_chunks_output_over_the_queries_and_falling_starts():
+    for q_lens, kv_lens in (([1, 7, 33], [30000, 9000, 20000]), ([300, 2, 1], [900, 130, 64])):
+        c = _Case(28, q_lens, kv_lens, 8, 1, 128, 16, "bf16")
+        want = c.run()
+        assert c.run(out=c.q) is c.q and torch.equal(c.q, want)
+    from kessie_b200 import _lib, ops
+    c.start = _i32([0, 300, 1, 303])
+    out = torch.full_like(want, 7.0)
+    c.run(out=out)
+    assert ops.read_device_status() == _lib.DEV_BAD_ARG and (out == 7.0).all()
+    with pytest.raises(Exception, match="share memory"):
+        c.run(out=out[:1].expand_as(out))
+
+
+@pytest.mark.parametrize("window", [140, 150, 2 ** 31 - 1])
+def test_chunks_window_wider_than_the_sequences(window):
+    """No less than causal attention, with more queries than keys too."""
+    c = _Case(29, [200, 3], [140, 130], 8, 2, 128, 16, "bf16")
+    want = c.run()
+    c.check(want)
+    for causal in (True, False):
+        assert torch.equal(c.run(window_size=window, causal=causal, max_seq_len=140), want)
+
+
+def test_conversions_run_on_the_given_stream():
+    """64-bit lengths, positions and slots and an unaligned q are converted in
+    the given stream's order, not behind the work of the current one."""
+    from kessie_b200 import ops
+    c = _Case(30, [1, 20], [300, 400], 8, 2, 128, 16, "bf16")
+    want = c.run()
+    flat = torch.zeros(21 * 8 * 128 + 1, dtype=torch.bfloat16, device="cuda")
+    c.q = flat[1:].view(21, 8, 128).copy_(c.q)
+    c.start, c.seq, c.bt = c.start.long(), c.seq.long(), c.bt.long()
+    k = torch.randn(21, 2, 128, device="cuda")
+    pos = torch.arange(63, device="cuda").view(3, 21)
+    turned = ops.rope_axes_remap(k, None, pos, [16, 24, 24], out=torch.empty_like(k))
+    R = 2
+    free, table = torch.arange(40, device="cuda"), torch.full((R, 30), -1, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([5, 40], device="cuda")
+    tables = ops.step_tables(torch.zeros_like(lens), lens, table.clone(), 16, free, 45)
+    zeros = torch.zeros_like(lens)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    busy = torch.cuda.Event()
+    torch.cuda._sleep(400_000_000)                                    # the current stream is busy for a while
+    busy.record()
+    got = c.run(stream=s)
+    gk = ops.rope_axes_remap(k, None, pos, [16, 24, 24], out=torch.empty_like(k), stream=s.cuda_stream)
+    gt = ops.step_tables(zeros, lens, table, 16, free, 45, stream=s)
+    s.synchronize()
+    assert not busy.query()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(gk, turned)
+    assert all(torch.equal(a, b) for a, b in zip(gt, tables))
+
+
 # ------------------------------------------------------------------ a step of all three
 @pytest.mark.parametrize("captured", [False, True])
 def test_step_of_all_three(captured):

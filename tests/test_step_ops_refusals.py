@@ -113,3 +113,32 @@ def test_wrappers_refuse_host_tensors():
     c = torch.zeros(4, 16, 4, 128)
     with pytest.raises(ValueError, match="CUDA"):
         ops.paged_fog_chunks(x, c, c, torch.zeros(1, 4, dtype=torch.int32), i, i[:1])
+
+
+def _buffers():
+    return {n: ctypes.addressof(b) for n, b in _KEEP.items()}
+
+
+_KEEP = {n: (ctypes.c_int64 * 64)() for n in ("ctx", "new", "table", "free", "count", "start", "seq", "pos", "slots",
+                                             "used")}
+
+
+@pytest.mark.parametrize("output,source", [("seq", "ctx"), ("seq", "new"), ("start", "ctx"), ("used", "count"),
+                                           ("pos", "free"), ("slots", "new"), ("table", "free")])
+def test_step_tables_refuses_outputs_in_its_inputs(lib, output, source):
+    """The inputs are read by every block while another writes: last step's
+    seq_lens cannot be the context lengths of a call that writes them."""
+    at = _buffers()
+    at[output] = at[source]
+    assert _tables(lib, **at) == ARG and "shares memory" in _msg(), _msg()
+    at[output] = at[source] + 4                                       # one element on
+    if output not in ("used",):
+        assert _tables(lib, **at) == ARG and "shares memory" in _msg(), _msg()
+
+
+def test_outputs_whose_rows_share_memory_are_refused(lib):
+    sec = (ctypes.c_int * 1)(64)
+    for st, sh in ((0, 128), (256, 0)):
+        assert lib.kessie_rope_axes_remap_v2(16, 256, 128, 16, st, sh, 1, 4, 2, 128, None, 0, 16, 4, sec, 1, 0, 1e4,
+                                             None) == ARG
+        assert "share memory" in _msg()
