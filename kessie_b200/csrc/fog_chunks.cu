@@ -49,7 +49,7 @@
 //
 // Bound by: the serial chain scores -> exponentials -> P -> product of chunks
 // (tensor pipe 60 %, MUFU 61 % busy; 4,096 tokens of 32 / 8 heads of 128 over
-// 131,072 keys, bf16: 6.9 ms = 1,250 TFLOP/s, 9.2 ms with the V fog, where the
+// 131,072 keys, bf16: 6.9 ms = 1,250 TFLOP/s, 9.0 ms with the V fog, where the
 // power cap holds the clock near 1.75 GHz), HBM for decodes (28 of 1k-16k keys:
 // 6.0 TB/s, every key read once), launches and the plan for the smallest (17 us).
 //
@@ -503,7 +503,9 @@ __device__ __forceinline__ float softmax_p(const uint32_t (&sv)[4][32], uint32_t
                                            const float* wts, uint64_t* half_bar) {
     const uint64_t sc2 = ptx::f2_pack(scale, scale), nb2 = ptx::f2_pack(nb, nb);
     uint64_t sum[2] = {0ull, 0ull};
-    constexpr int kAhead = 1;
+    // quads of weights on their way: 1 ahead 1,073 us, 4 1,037, 6 1,014, 8 1,065, 12 1,037 (2,048 tokens over 32,768
+    // keys); the score fog's reads show no difference between 1 and 8
+    constexpr int kAhead = 6;
     const uint32_t wa = WEIGHTED ? ptx::smem_u32(wts) : 0u;
     ulonglong2 w[kAhead];
     if (WEIGHTED)
