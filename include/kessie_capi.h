@@ -640,7 +640,8 @@ int kessie_rope_axes_insert_v2(const void* q, int64_t q_token_stride, int64_t q_
  * scaled scores, by key position, kv_len = the sequence's keys); both nullable,
  * not both at once.
  * Rows that see no key are 0; rows of no sequence (a padded batch) are left as
- * they were.  Keys that no row of a sequence sees are never used, so their
+ * they were.  A query whose scores come out NaN, or infinite above, gives a NaN
+ * row and changes no other.  Keys that no row of a sequence sees are never used, so their
  * pages may hold anything; keys that some of its rows see must be finite.
  * A page id outside [0, num_pages) reads as zero keys and values and records
  * KESSIE_DEV_BAD_PAGE_ID; a length past max_seq_len, or offsets that leave

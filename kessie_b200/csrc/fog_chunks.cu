@@ -1101,7 +1101,9 @@ __global__ void __launch_bounds__(256) fog_chunks_merge_kernel(const ChunkParams
         }
         m = top;
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    // only a row without keys has l = 0.  A row whose scores are NaN (its query is not finite) has a NaN l beside a
+    // maximum of -inf (maxima pass NaN over), which the factors above would drop: it stays NaN, as in an uncut tile
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     uint32_t pk[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) pk[i] = ptx::pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
