@@ -454,7 +454,7 @@ template <int FOG>
 __device__ __forceinline__ int fog_tiles(const ChunkParams& p, const Item& it, int edge) {
     if (FOG == kNoFog) return 0;
     if (FOG == kScoreFog && p.bias.recall) return it.n;
-    return min(it.n, max(0, (edge - it.key0 + 127) >> 7));
+    return edge <= it.key0 ? 0 : min(it.n, ((edge - it.key0 - 1) >> 7) + 1);     // holds for an edge of INT_MAX
 }
 // First key past the fog of a sequence.
 template <int FOG>
@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
             // fog weights of key tile t, two tiles ahead of its V: that V's stage was free, so this slot is
             const int edge = is_k ? 0 : fog_edge<FOG>(p, it.b, it.kv);
             const int nw = is_k ? 0 : fog_tiles<FOG>(p, it, edge);
-            const float inv_den = 1.f / (float)max(edge - 1, 1);
+            const float inv_den = 1.f / (float)(max(edge, 2) - 1);
             const double inv_fb = FOG == kScoreFog ? 1.0 / (double)(float)max(edge, 1) : 0.0;
             auto weights = [&](int t) {
                 if (FOG == kNoFog || t >= nw) return;

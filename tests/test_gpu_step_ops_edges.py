@@ -1,6 +1,6 @@
 """GPU: calls of the scheduler-step operators at the edges of what they allow:
 queries that are not finite, against the rule that a row's values reach that
-row alone."""
+row alone, and the ends of int32 in the fog's boundary, against 64 bits."""
 
 import pytest
 import torch
@@ -66,3 +66,15 @@ def test_chunks_rows_without_keys_are_zero_whatever_their_queries(dt):
     assert out[:150].count_nonzero() == 0 and out[200:].count_nonzero() == 0
     clean = _Case(72, [200, 3], [50, 0], 8, 2, 128, 16, dt)
     assert torch.equal(out[150:200], clean.run()[150:200])
+
+
+# ------------------------------------------------------------------ the fog's boundary
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("clear", [2 ** 31 - 1, 2 ** 31 - 127, 2 ** 31 - 128, -2 ** 31, 1, 2])
+def test_chunks_fog_boundary_anywhere_in_int32(clear, dt):
+    """All keys fogged, far past the last of them, or none: single and pair
+    tiles, cut ones among them (pieces from key 0 and from later keys)."""
+    q_lens, kv_lens = [1, 70, 3, 200], [5000, 300, 40, 9000]
+    c = _Case(73, q_lens, kv_lens, 8, 2, 64, 16, dt)
+    c.check(c.run(clear_start=_i32([clear] * 4), fog_alpha=0.02), clear=[min(max(clear, 0), 2 ** 31 - 1)] * 4,
+            alpha=0.02)
