@@ -74,6 +74,11 @@ constexpr int kMaxBatch = 8192;              // sequences whose prefix sums the 
 constexpr int kWStages = 4;                  // key tiles of fog weights in flight
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;    // log2 units the running max may lag behind
+// P is rounded to the 16-bit type of V for the product (relative 2^-11 in fp16, 2^-8 in bf16; the row sum takes it
+// unrounded).  In fp16 a small P is also subnormal, off by 2^-25, and over 131,072 keys these add up to 2^-8 of the
+// largest value (one key against 131,071 of e^-16.25 each lost a quarter of what those bring).  So fp16 holds P times
+// 2^7, which with the lag above stays within 2^15; the factor is in l and O alike and leaves with 1 / l.
+constexpr float kHalfHeadroom = 7.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kProducerRegs = 88;
 static_assert(256 * kSoftmaxRegs + 128 * kProducerRegs <= kThreads * kLaunchRegs, "register split exceeds the pool");
@@ -495,9 +500,10 @@ __device__ __forceinline__ void lds_quad(ulonglong2& w, uint32_t saddr) {
     asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(w.x), "=l"(w.y) : "r"(saddr));
 }
 
-// p = 2^(s * scale + nb) of one row's 128 scores, packed to 16-bit pairs over
-// the first 64 columns of the row's S; FOG == kValueFog with `wts`: p * w is
-// packed.  Returns the row sum of the unweighted, unrounded p.
+// p = 2^(s * scale + nb) of one row's 128 scores (nb: minus the reference, plus
+// fp16's headroom), packed to 16-bit pairs over the first 64 columns of the
+// row's S; FOG == kValueFog with `wts`: p * w is packed.  Returns the row sum of
+// the unweighted, unrounded p.
 template <bool BF16, bool WEIGHTED>
 __device__ __forceinline__ float softmax_p(const uint32_t (&sv)[4][32], uint32_t sreg, float scale, float nb,
                                            const float* wts, uint64_t* half_bar) {
@@ -914,7 +920,7 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                         l *= factor;
                         m_used = m_tile;
                     }
-                    const float nb = m_used == -INFINITY ? 0.f : -m_used;
+                    const float nb = m_used == -INFINITY ? 0.f : (BF16 ? 0.f : kHalfHeadroom) - m_used;
                     const bool moved = __any_sync(0xffffffffu, need && old != -INFINITY);
                     // O moves with the reference (rare): its last product is complete, the next waits for P
                     if (moved) {

@@ -1,11 +1,12 @@
 """GPU: calls of the scheduler-step operators at the edges of what they allow:
 queries that are not finite, against the rule that a row's values reach that
-row alone, and the ends of int32 in the fog's boundary, against 64 bits."""
+row alone; the ends of int32 in the fog's boundary and sums of very many small
+probabilities, against 64 bits."""
 
 import pytest
 import torch
 
-from tests.test_gpu_step_ops import _Case, _i32
+from tests.test_gpu_step_ops import DT, _Case, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +79,41 @@ def test_chunks_fog_boundary_anywhere_in_int32(clear, dt):
     c = _Case(73, q_lens, kv_lens, 8, 2, 64, 16, dt)
     c.check(c.run(clear_start=_i32([clear] * 4), fog_alpha=0.02), clear=[min(max(clear, 0), 2 ** 31 - 1)] * 4,
             alpha=0.02)
+
+
+# ------------------------------------------------------------------ many small probabilities
+@pytest.mark.parametrize("fog", ["none", "values"])
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_chunks_many_small_probabilities_add_up(dt, fog):
+    """One key takes nearly all of a row, 131,071 others e^-16.25 each: 1.1 % of
+    the output together.  The chunk is long enough that a block goes through
+    all keys of a tile in one piece, with the maximum from the first key tile.
+
+    P is held in 16 bits: relative h, and in fp16 an absolute 2^-25 of the 2^7
+    that the largest probability is held at, 2^-32 a key of the row's maximum.
+    The scores are exact here (one product each); the exponent's fp32 rounding
+    (2^-24 of 23) and the exponential are good to 1e-5."""
+    from kessie_b200 import ops
+    S, T, H, D, ps = 131072, 4864, 8, 64, 64
+    pages = S // ps
+    kv = torch.zeros(pages, ps, 2, H, D, dtype=DT[dt], device="cuda")
+    kv[0, 0, 0, :, 0] = 16.25
+    kv[:, :, 1] = 1.0
+    kv[0, 0, 1] = 0.0
+    q = torch.zeros(T, H, D, dtype=DT[dt], device="cuda")
+    q[:, :, 0] = 8.0                                                  # score 8 * 16.25 / sqrt(64)
+    clear = S // 2
+    got = ops.paged_fog_chunks(q, kv[:, :, 0], kv[:, :, 1], torch.arange(pages, device="cuda").int()[None],
+                               _i32([0, T]), _i32([S]), clear_start=_i32([clear]) if fog == "values" else None,
+                               fog_alpha=0.5)
+    j = torch.arange(S, dtype=torch.float64, device="cuda")
+    w = torch.where(j < clear, (j / (clear - 1)).sqrt(), 1.0) if fog == "values" else torch.ones_like(j)
+    w[0] = 0.0                                                        # that key's value
+    p = torch.arange(S - T, S, device="cuda")
+    small = torch.tensor(-16.25, dtype=torch.float64, device="cuda").exp()
+    den = 1 + p * small
+    want = (torch.cumsum(w, 0)[p] * small / den)[:, None, None]
+    h = torch.finfo(DT[dt]).eps / 2
+    tol = want * (2.01 * h + 2e-5) + (S * 2.0 ** -32 if dt == "fp16" else 0.0)
+    err = (got.double() - want).abs()
+    assert (err <= tol).all(), f"worst {err.max().item()} at {want.min().item()} .. {want.max().item()}"
