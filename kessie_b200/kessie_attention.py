@@ -210,6 +210,20 @@ class KeSSieAttentionImpl:
                                        output_block_scale)
         return self._fog_forward(query, kv_cache, attn_metadata, output, state)
 
+    @staticmethod
+    def _check_lengths(md, capacity):
+        """Raise for a request of several new tokens that is longer than its
+        row of the block table.  Called where vLLM's bound on the lengths is
+        above the row's, so that the lengths themselves are read by the host
+        only then (in a capture they cannot be: the kernel cuts them and
+        records it in the device status)."""
+        if torch.cuda.is_current_stream_capturing():
+            return
+        starts, lens = md.query_start_loc.tolist(), md.seq_lens.tolist()
+        for first, end, n in zip(starts, starts[1:], lens):
+            if end - first > 1 and n > capacity:
+                raise ValueError(f"max_kv_len {n} exceeds the block table capacity {capacity}")
+
     def _fog_forward(self, query, kv_cache, md, output, state):
         n = int(md.num_actual_tokens)
         Hq, D = self._num_heads, self._head_size
@@ -224,6 +238,9 @@ class KeSSieAttentionImpl:
             return output
         # a mixed step (prompt chunks, drafts, decodes): one call for the batch, lengths read on the device
         B = sl.shape[0]
+        capacity = bt.shape[1] * key_cache.shape[1]
+        if (getattr(md, "max_seq_len", None) or 0) > capacity:
+            self._check_lengths(md, capacity)
         ops.paged_fog_chunks(q, key_cache, value_cache, bt[:B], md.query_start_loc[:B + 1], sl, out=out, **kw)
         return output
 

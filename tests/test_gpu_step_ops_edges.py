@@ -1,7 +1,9 @@
 """GPU: calls of the scheduler-step operators at the edges of what they allow:
 queries that are not finite, against the rule that a row's values reach that
 row alone; the ends of int32 in the fog's boundary and sums of very many small
-probabilities, against 64 bits."""
+probabilities, against 64 bits; and the mixed steps of the vLLM attention."""
+
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -117,3 +119,44 @@ def test_chunks_many_small_probabilities_add_up(dt, fog):
     tol = want * (2.01 * h + 2e-5) + (S * 2.0 ** -32 if dt == "fp16" else 0.0)
     err = (got.double() - want).abs()
     assert (err <= tol).all(), f"worst {err.max().item()} at {want.min().item()} .. {want.max().item()}"
+
+
+# ------------------------------------------------------------------ the vLLM attention's mixed steps
+@pytest.fixture
+def fog_on():
+    from kessie_b200 import kessie_attention as A
+    A.KESSIE_STATE.update(fog_alpha=1.5, fog_start=0.5, prompt_len=10, recall_positions=[], recall_boost=0.0)
+    A.KESSIE_STATE.enabled = True
+    yield A
+    A.KESSIE_STATE.update(prompt_len=0)
+
+
+class _Step:
+    """A vLLM step of KeSSieAttentionImpl over a _Case's cache."""
+
+    def __init__(self, A, c, **metadata):
+        Hq, D = c.q.shape[1:]
+        inner = SimpleNamespace(num_heads=Hq, num_kv_heads=c.k.shape[2], head_size=D, scale=D ** -0.5,
+                                sliding_window=None)
+        self.impl, self.c, self.cache = A.KeSSieAttentionImpl(_inner_impl=inner), c, torch.stack([c.k, c.v])
+        self.md = SimpleNamespace(num_actual_tokens=sum(c.q_lens), max_query_len=max(c.q_lens),
+                                  query_start_loc=c.start, seq_lens=c.seq, block_table=c.bt,
+                                  max_seq_len=max(c.kv_lens), **metadata)
+        self.out = torch.full((c.q.shape[0], Hq * D), 2.0, dtype=c.q.dtype, device="cuda")
+
+    def forward(self):
+        assert self.impl.forward(None, self.c.q, None, None, self.cache, self.md, self.out) is self.out
+        return self.out.view(self.c.q.shape)
+
+
+def test_vllm_mixed_step_refuses_a_length_past_the_block_table(fog_on):
+    """As the call per request did: an error, not a device status bit that the
+    attention never reads.  A bound above the table alone is no error."""
+    c = _Case(74, [1, 60, 7], [900, 300, 77], 8, 2, 128, 16, "bf16", layout="vllm")
+    step = _Step(fog_on, c)
+    want = step.forward().clone()
+    step.md.max_seq_len = 10 ** 6                                     # vLLM's bound: every length fits all the same
+    assert torch.equal(step.forward(), want)
+    c.seq[1] = step.md.max_seq_len = c.bt.shape[1] * 16 + 1
+    with pytest.raises(ValueError, match="capacity"):
+        step.forward()
