@@ -28,7 +28,7 @@ struct DecodeF32Args {
     float sm_scale;
     int B, Hq, Hkv, D, max_seq_len;
     unsigned long long* counters; // [B*Hkv]
-    uint32_t tag;                 // non-zero per-launch tag of the arrival counters
+    uint64_t tag;                 // per-launch tag of the arrival counters (upper 48 bits)
     float* part_ml;               // [slots][G][2]
     float* part_o;                // [slots][G][D]
     int slots;

@@ -103,8 +103,8 @@ struct DecodeParams {
     int units_per_page, num_pages, max_units;
     float* part_o;        // [slots][G][D]   segment partial O/l
     float* part_ml;       // [slots][G][2]   (m in log2 units, l)
-    unsigned long long* counters;   // [B*Hkv] (launch tag << 32) | arrivals, per group
-    uint32_t tag;         // this launch's tag (non-zero); a counter with another tag counts as zero
+    unsigned long long* counters;   // [B*Hkv] launch tag | arrivals, per group
+    uint64_t tag;         // this launch's tag, in the upper 48 bits; a counter with another tag counts as zero
     void* out;            // [B][Hq][D] q dtype, or null
     float* out_part;      // [B][Hq][D+2] (O/l, ln m, l), or null
     CpLink cp;            // cp.world > 0: push merged rows into every rank's exchange buffer
@@ -321,13 +321,12 @@ __device__ void merge_and_emit(const DecodeParams& p, int g, int first, int K, i
 
 // Count one arrival at a group counter; returns the arrivals before this one
 // (a counter holding another launch's tag, or garbage, counts as zero).
-__device__ __forceinline__ unsigned arrive(unsigned long long* c, uint32_t tag) {
-    const unsigned long long hi = (unsigned long long)tag << 32;
+__device__ __forceinline__ unsigned arrive(unsigned long long* c, uint64_t tag) {
     unsigned long long old = *reinterpret_cast<volatile unsigned long long*>(c);
     while (true) {
-        const unsigned long long cur = (old >> 32) == tag ? old : hi;
+        const unsigned long long cur = (old & ~0xffffull) == tag ? old : tag;
         const unsigned long long prev = atomicCAS(c, old, cur + 1ull);
-        if (prev == old) return (unsigned)(cur & 0xffffffffull);
+        if (prev == old) return (unsigned)(cur & 0xffffull);      // at most one arrival a CTA
         old = prev;
     }
 }
@@ -1080,10 +1079,11 @@ int prepare_decode(DecodeParams& p, Plan& pl, const void* q, int64_t q_stride_b,
     p.max_units = pl.max_units;
     char* ws = static_cast<char*>(workspace);
     p.counters = reinterpret_cast<unsigned long long*>(ws + pl.cnt_off);
-    static std::atomic<uint32_t> launch_tag{0};
-    uint32_t tag = ++launch_tag;
-    if (tag == 0) tag = ++launch_tag;
-    p.tag = tag;
+    // A tag of its own for each launch (an odd factor permutes the 48-bit numbers), and one that the words of a
+    // workspace do not hold by chance: the launch number itself is the upper half of many an int64 or pair of int32,
+    // and a counter left with it lost its group's merge.
+    static std::atomic<uint64_t> launches{0};
+    p.tag = (++launches * 0x9e3779b97f4a7c15ull) << 16;
     p.part_ml = reinterpret_cast<float*>(ws + pl.ml_off);
     p.part_o = reinterpret_cast<float*>(ws + pl.o_off);
     p.status = device_status_ptr();

@@ -139,13 +139,12 @@ __device__ __forceinline__ float fog_weight_f32(const DecodeF32Args& p, int cs, 
 
 // Count one arrival at a group counter; returns the arrivals before this one
 // (a counter holding another launch's tag counts as zero).
-__device__ __forceinline__ unsigned arrive_tagged(unsigned long long* c, uint32_t tag) {
-    const unsigned long long hi = (unsigned long long)tag << 32;
+__device__ __forceinline__ unsigned arrive_tagged(unsigned long long* c, uint64_t tag) {
     unsigned long long old = *reinterpret_cast<volatile unsigned long long*>(c);
     while (true) {
-        const unsigned long long cur = (old >> 32) == tag ? old : hi;
+        const unsigned long long cur = (old & ~0xffffull) == tag ? old : tag;
         const unsigned long long prev = atomicCAS(c, old, cur + 1ull);
-        if (prev == old) return (unsigned)(cur & 0xffffffffull);
+        if (prev == old) return (unsigned)(cur & 0xffffull);      // one arrival a slot
         old = prev;
     }
 }
