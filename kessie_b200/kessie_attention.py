@@ -241,7 +241,9 @@ class KeSSieAttentionImpl:
         capacity = bt.shape[1] * key_cache.shape[1]
         if (getattr(md, "max_seq_len", None) or 0) > capacity:
             self._check_lengths(md, capacity)
-        ops.paged_fog_chunks(q, key_cache, value_cache, bt[:B], md.query_start_loc[:B + 1], sl, out=out, **kw)
+        for b in range(0, B, ops.MAX_CHUNK_SEQUENCES):                   # one call, but for the largest batches
+            e = min(b + ops.MAX_CHUNK_SEQUENCES, B)
+            ops.paged_fog_chunks(q, key_cache, value_cache, bt[b:e], md.query_start_loc[b:e + 1], sl[b:e], out=out, **kw)
         return output
 
 

@@ -758,6 +758,9 @@ def rope_axes_insert(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, position
     return out_q
 
 
+MAX_CHUNK_SEQUENCES = 8192      # sequences of one paged_fog_chunks call
+
+
 def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                      query_start_loc: torch.Tensor, seq_lens: torch.Tensor, clear_start=None, fog_alpha: float = 0.5,
                      window_size: int = 0, causal: bool = True, sm_scale: Optional[float] = None,
@@ -774,6 +777,7 @@ def paged_fog_chunks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     views, block_table [B, maxP].  causal=False without a window attends to
     all of the sequence's keys, whatever the number of queries (cross
     attention).  clear_start / fog_alpha or bias as in paged_fog_decode.
+    At most MAX_CHUNK_SEQUENCES sequences a call.
     Returns out [T, Hq, D] (which may be q itself); rows that see no key are 0,
     rows of no sequence (a padded batch) are not written, and none when
     query_start_loc falls.  Scratch memory: one buffer per stream, a

@@ -160,3 +160,31 @@ def test_vllm_mixed_step_refuses_a_length_past_the_block_table(fog_on):
     c.seq[1] = step.md.max_seq_len = c.bt.shape[1] * 16 + 1
     with pytest.raises(ValueError, match="capacity"):
         step.forward()
+
+
+def _fog_bias_16(dt, recalled=()):
+    """kv_len -> the step's bias, rounded to the 16-bit type at each operation as torch rounds it."""
+    r = lambda x: x.to(DT[dt]).float()
+
+    def bias(s):
+        j, fb = torch.arange(s, device="cuda"), int(s * 0.5)
+        d = r(1.0 - r(r(j.float()) / max(fb, 1)))
+        x = torch.where(j < fb, r(r(d * d) * -1.5), 0.0).double()
+        for p in recalled:
+            if p < s:
+                x[p] = 0.25
+        return x
+    return bias
+
+
+def test_vllm_mixed_step_of_more_sequences_than_one_call_takes(fog_on):
+    from kessie_b200 import ops
+    B = ops.MAX_CHUNK_SEQUENCES + 5
+    q_lens = [1 if i % 100 else 3 for i in range(B)]
+    q_lens[ops.MAX_CHUNK_SEQUENCES - 2:ops.MAX_CHUNK_SEQUENCES + 2] = [2, 40, 1, 70]     # around the border
+    kv_lens = [n + i % 37 for i, n in enumerate(q_lens)]
+    c = _Case(75, q_lens, kv_lens, 4, 1, 64, 16, "bf16", layout="vllm", pad=3)
+    step = _Step(fog_on, c)
+    got = step.forward()
+    assert (got[sum(q_lens):] == 2.0).all()
+    c.check(got, bias=_fog_bias_16("bf16"))
