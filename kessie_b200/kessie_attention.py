@@ -29,7 +29,7 @@ from __future__ import annotations
 import logging
 import os
 import threading
-from typing import Optional, Set
+from typing import NamedTuple, Optional, Sequence, Set, Tuple
 
 import torch
 
@@ -153,11 +153,40 @@ _BIAS_CACHE = _BiasCache()
 _FOG_CACHE = _FogCache()
 
 
+class QueryRun(NamedTuple):
+    """Neighbouring requests [first, end) of a step, from row `row` of its
+    tokens on, that all have one new token (decodes) or none of which has."""
+    first: int
+    end: int
+    row: int
+    decodes: bool
+
+
+def query_runs(starts: Sequence[int]) -> Tuple[QueryRun, ...]:
+    """The runs of a step, from the offsets of its requests' tokens."""
+    runs = []
+    for i in range(len(starts) - 1):
+        one = starts[i + 1] - starts[i] == 1
+        if runs and runs[-1].decodes == one:
+            runs[-1] = runs[-1]._replace(end=i + 1)
+        else:
+            runs.append(QueryRun(i, i + 1, starts[i], one))
+    return tuple(runs)
+
+
+# A mixed step's decodes go to the paged decode, apart from its chunks, when there is one run of each and the decodes
+# have at least this many (request, KV head) pairs an SM: the ragged call pays for the start and end of each of those
+# tiles, which few of them hide in the chunks' time and many do not.  GPU time a layer, one call against two (bf16,
+# 32 / 8 heads of 128): 64 decodes over 2,000 keys + a prompt of 512 150 against 126 us, 256 over 500 + 512 209 / 162,
+# 64 over 32,000 + 2,048 1,576 / 1,336; 32 over 500 + 512 58 / 72, 16 over 8,000 + 16 105 / 112.
+_SPLIT_TILES = 3
+
+
 class KeSSieAttentionImpl:
     """Per-layer attention: with the fog active, a decode step runs in the paged
     decode and any other step (prompt chunks, drafts, decodes mixed) in one
-    ragged-chunk call, neither reading a length back to the host, with the fog
-    bias applied to the scores;
+    ragged-chunk call, or with many decodes in one call of each, none reading a
+    length back to the host, with the fog bias applied to the scores;
     otherwise (fog off, profiling run, features the kernels do not cover) the
     wrapped vLLM implementation runs.  Attributes and methods not defined here
     (e.g. the KV-cache write) are the wrapped implementation's."""
@@ -236,15 +265,36 @@ class KeSSieAttentionImpl:
         if int(md.max_query_len) == 1:                 # decode step: one launch for the batch
             ops.paged_fog_decode(q, key_cache, value_cache, bt[:n], sl[:n], out=out, **kw)
             return output
-        # a mixed step (prompt chunks, drafts, decodes): one call for the batch, lengths read on the device
+        # a mixed step (prompt chunks, drafts, decodes): one call for the batch, or two; lengths read on the device
         B = sl.shape[0]
         capacity = bt.shape[1] * key_cache.shape[1]
         if (getattr(md, "max_seq_len", None) or 0) > capacity:
             self._check_lengths(md, capacity)
-        for b in range(0, B, ops.MAX_CHUNK_SEQUENCES):                   # one call, but for the largest batches
-            e = min(b + ops.MAX_CHUNK_SEQUENCES, B)
-            ops.paged_fog_chunks(q, key_cache, value_cache, bt[b:e], md.query_start_loc[b:e + 1], sl[b:e], out=out, **kw)
+        for run in self._launches(md, B, capacity, key_cache.shape[1]):
+            if run.decodes:
+                rows, reqs = slice(run.row, run.row + run.end - run.first), slice(run.first, run.end)
+                ops.paged_fog_decode(q[rows], key_cache, value_cache, bt[reqs], sl[reqs], out=out[rows], **kw)
+                continue
+            for b in range(run.first, run.end, ops.MAX_CHUNK_SEQUENCES):     # one call, but for the largest batches
+                e = min(b + ops.MAX_CHUNK_SEQUENCES, run.end)
+                ops.paged_fog_chunks(q, key_cache, value_cache, bt[b:e], md.query_start_loc[b:e + 1], sl[b:e], out=out,
+                                     **kw)
         return output
+
+    def _launches(self, md, B, capacity, page_size):
+        """The calls of a mixed step of B requests: all of them in one
+        ragged-chunk call, or the decodes apart in the paged decode.  The
+        latter takes the metadata builder's host copy of the offsets; a capture
+        holds for other offsets too, and is one call."""
+        runs = getattr(md, "query_runs", None)
+        whole = (QueryRun(0, B, 0, False),)
+        if not runs or len(runs) != 2 or runs[-1].end != B or torch.cuda.is_current_stream_capturing():
+            return whole
+        tiles = sum(r.end - r.first for r in runs if r.decodes) * self._num_kv_heads
+        sms = torch.cuda.get_device_properties(md.seq_lens.device).multi_processor_count
+        if tiles < _SPLIT_TILES * sms or page_size > 256 or tiles * (capacity // 16) > 1 << 30:  # the decode's limits
+            return whole
+        return runs
 
 
 # ----------------------------------------------------------------- vLLM registration
@@ -272,6 +322,21 @@ if HAS_VLLM:
         @staticmethod
         def get_impl_cls():
             return KeSSieAttentionImpl
+
+        @staticmethod
+        def get_builder_cls():
+            return KeSSieMetadataBuilder
+
+    class KeSSieMetadataBuilder(_FlashAttentionBackend.get_builder_cls()):
+        """FlashAttention's builder; the metadata of a mixed step carries its
+        runs of decodes and chunks, from vLLM's host copy of the offsets."""
+
+        def build(self, common_prefix_len, common_attn_metadata, fast_build=False):
+            md = super().build(common_prefix_len, common_attn_metadata, fast_build)
+            starts = getattr(common_attn_metadata, "query_start_loc_cpu", None)
+            if starts is not None and common_attn_metadata.max_query_len > 1:
+                md.query_runs = query_runs(starts.tolist())
+            return md
 else:
     class KeSSieAttentionBackend:                      # pragma: no cover
         pass

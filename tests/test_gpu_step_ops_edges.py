@@ -188,3 +188,46 @@ def test_vllm_mixed_step_of_more_sequences_than_one_call_takes(fog_on):
     got = step.forward()
     assert (got[sum(q_lens):] == 2.0).all()
     c.check(got, bias=_fog_bias_16("bf16"))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("order", ["decodes first", "chunks first"])
+def test_vllm_mixed_step_of_many_decodes(fog_on, monkeypatch, order, dt):
+    """One run of decodes and one of chunks (requests without new tokens among
+    them): a call of each, the rows of both as in the 64-bit run; the same step
+    captured is one call, which holds for other lengths."""
+    A = fog_on
+    A.KESSIE_STATE.update(recall_positions=[3, 250, 700], recall_boost=0.25)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    Hkv = 8
+    many = -(-3 * sms // Hkv) + 1
+    decodes, chunks = [1] * many, [60, 0, 7, 200]
+    q_lens = decodes + chunks if order == "decodes first" else chunks + decodes
+    kv_lens = [n + 17 * i % 900 for i, n in enumerate(q_lens)]
+    c = _Case(76, q_lens, kv_lens, 16, Hkv, 64, 16, dt, layout="vllm", pad=5)
+    step = _Step(A, c, query_runs=A.query_runs(c.start.tolist()))
+    calls = []
+    for name in ("paged_fog_decode", "paged_fog_chunks"):
+        def spy(*a, _f=getattr(A.ops, name), _name=name, **kw):
+            calls.append(_name)
+            return _f(*a, **kw)
+        monkeypatch.setattr(A.ops, name, spy)
+    bias = _fog_bias_16(dt, [3, 250, 700])
+    got = step.forward()
+    assert sorted(calls) == ["paged_fog_chunks", "paged_fog_decode"]
+    assert (got[sum(q_lens):] == 2.0).all()
+    c.check(got, bias=bias)
+    del calls[:]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step.forward()
+    assert calls == ["paged_fog_chunks"]
+    c.q_lens = q_lens[::-1]
+    c.kv_lens = [max(s - 5, 0) for s in kv_lens]                      # some with fewer keys than new tokens
+    c.start.copy_(_i32([sum(c.q_lens[:i]) for i in range(len(q_lens) + 1)]))
+    c.seq.copy_(_i32(c.kv_lens))
+    step.out.fill_(2.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (got[sum(q_lens):] == 2.0).all()
+    c.check(got, bias=bias)
