@@ -302,6 +302,8 @@ int fill_table(RopeAxesTable* tab, const int* sections, int axes, int interleave
         tab->axis[d] = (uint8_t)a;
         ++count[a];
         const float f = (float)pow((double)theta, -(double)d / half);
+        if (isinf(f))                    // theta below about 1e-39: no fraction of a turn
+            return set_error(KESSIE_ERR_ARG, "rope_axes: theta %g: frequency %d is past fp32", (double)theta, d);
         const long double turns = (long double)f / 6.283185307179586476925286766559L;
         long double frac = turns - floorl(turns);
         tab->turn[d] = (uint64_t)(frac * 0x1p64L);
