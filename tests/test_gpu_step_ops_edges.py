@@ -1,7 +1,8 @@
 """GPU: calls of the scheduler-step operators at the edges of what they allow:
 queries that are not finite, against the rule that a row's values reach that
 row alone; the ends of int32 in the fog's boundary and sums of very many small
-probabilities, against 64 bits; and the mixed steps of the vLLM attention."""
+probabilities; plans that begin with whole tiles; the types' lowest values, all
+against 64 bits; and the mixed steps of the vLLM attention."""
 
 from types import SimpleNamespace
 
@@ -231,3 +232,80 @@ def test_vllm_mixed_step_of_many_decodes(fog_on, monkeypatch, order, dt):
     torch.cuda.synchronize()
     assert (got[sum(q_lens):] == 2.0).all()
     c.check(got, bias=bias)
+
+
+# ------------------------------------------------------------------ whole tiles first
+def _whole_tiles(q_lens, kv_lens, Hq, Hkv, window=0, causal=True):
+    """(whole tiles a block takes first, tiles left to cut, single tiles) of the
+    plan, restated: tiles of 2 * (128 / G) tokens; a key tile of 128 costs 3
+    (2 for a tile of one half) and a tile 7; whole tiles come first where a tile
+    costs 192 or more in the mean and (sequence, head) has at least 2 tiles."""
+    blocks = torch.cuda.get_device_properties(0).multi_processor_count
+    half = 128 // (Hq // Hkv)
+    cost = tiles = single = 0
+    for n, s in zip(q_lens, kv_lens):
+        for t0 in range(0, n, 2 * half):
+            m = min(n - t0, 2 * half)
+            first = s - n + t0
+            hi = max(0, min(s, first + m)) if causal or window else s
+            lo = min(max(first - window + 1, 0), hi) if window else 0
+            keys = max(1, -(-hi // 128) - lo // 128)
+            cost += Hkv * (keys * (2 if m <= half else 3) + 7)
+            tiles += Hkv
+            single += Hkv * (m <= half)
+    whole = min(tiles // blocks, 128) if cost >= 192 * tiles and tiles >= 2 * len(q_lens) * Hkv else 0
+    return whole, tiles - whole * blocks, single
+
+
+# name: (new tokens, keys, Hq, Hkv, D, window, causal), with 148 blocks
+WHOLE = {
+    "one a block, a few cut": ([608], [20000], 64, 8, 64, 0, True),
+    "one a block, none cut": ([1180], [20000], 32, 4, 128, 0, True),
+    "two a block, most of a third cut": ([900, 750], [20000, 15000], 64, 8, 64, 0, True),
+    "two a block, single tiles": ([700, 650, 8, 1], [20000, 30000, 9000, 12000], 64, 8, 64, 0, True),
+    "window": ([700, 300], [24000, 20000], 64, 8, 128, 9000, True),
+    "contexts far apart": ([300, 1200], [40000, 1200], 32, 8, 128, 0, True),
+    "cross attention": ([400, 500], [16000, 9000], 64, 8, 64, 0, False)}
+
+
+@pytest.mark.parametrize("fog", ["none", "values", "scores"])
+@pytest.mark.parametrize("name", list(WHOLE))
+def test_chunks_whole_tiles_first(name, fog):
+    """Long contexts shared by many tiles: each block takes whole tiles before
+    the rest is cut; into the queries themselves, too."""
+    from kessie_b200 import ops
+    q_lens, kv_lens, Hq, Hkv, D, window, causal = WHOLE[name]
+    whole, left, single = _whole_tiles(q_lens, kv_lens, Hq, Hkv, window, causal)
+    assert whole >= (2 if name.startswith("two") else 1), f"no case of whole tiles on this GPU: {whole}, {left}"
+    assert (left == 0) == name.endswith("none cut") and (single > 8 or "single" not in name)
+    c = _Case(77, q_lens, kv_lens, Hq, Hkv, D, 16, "fp16" if fog == "values" else "bf16")
+    clear = [n * 3 // 4 for n in kv_lens] if fog == "values" else None
+    kw = dict(window_size=window, causal=causal)
+    bias = None
+    if fog == "values":
+        kw.update(clear_start=_i32(clear), fog_alpha=0.7)
+    elif fog == "scores":
+        kw.update(bias=ops.FogBias(1.5, 0.4, [3, 250, 8000], 0.25, dtype=torch.float32), fog_alpha=0.0)
+
+        def bias(s):
+            j, fb = torch.arange(s, device="cuda", dtype=torch.float64), int(s * 0.6)
+            x = torch.where(j < fb, -1.5 * (1 - j / max(fb, 1)) ** 2, 0.0)
+            for p in (3, 250, 8000):
+                if p < s:
+                    x[p] = 0.25
+            return x
+    got = c.run(**kw)
+    c.check(got, clear=clear, alpha=0.7, window=window, causal=causal, bias=bias)
+    assert torch.equal(c.run(**kw), got)
+    assert c.run(out=c.q, **kw) is c.q and torch.equal(c.q, got)
+
+
+# ------------------------------------------------------------------ the lowest values
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_chunks_values_of_the_types_lowest_value(dt):
+    """A value row of the type's lowest value among others, under equal scores
+    (all probabilities are 1, so that no sum leaves fp32)."""
+    c = _Case(78, [1, 5, 40], [600, 70, 1200], 8, 2, 128, 16, dt, scale=0.0)
+    for b in range(3):
+        c.v[c.bt[b, 0], 0] = torch.finfo(DT[dt]).min
+    c.check(c.run())
