@@ -920,7 +920,7 @@ __global__ void __launch_bounds__(kThreads, 1) fog_chunks_kernel(const __grid_co
                         l *= factor;
                         m_used = m_tile;
                     }
-                    const float nb = m_used == -INFINITY ? 0.f : (BF16 ? 0.f : kHalfHeadroom) - m_used;
+                    const float nb = m_used == -INFINITY ? 0.f : BF16 ? -m_used : kHalfHeadroom - m_used;
                     const bool moved = __any_sync(0xffffffffu, need && old != -INFINITY);
                     // O moves with the reference (rare): its last product is complete, the next waits for P
                     if (moved) {
