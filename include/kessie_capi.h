@@ -594,7 +594,7 @@ int kessie_step_tables_v2(const int32_t* context_lens, const int32_t* query_lens
  * in blocks (interleaved 0), or frequency d to axis d % num_axes while
  * d < num_axes * sections[axis], else to axis 0 (interleaved 1; sections that
  * this does not fill are refused).  Pairs (d, d + half) are turned by
- * (target - orig)[axis(d)] * f_d, computed exactly (fixed-point turns);
+ * (target - orig)[axis(d)] * f_d, computed as fixed-point turns (to 2^-31 of one);
  * dimensions from 2 * half on pass through.  Positions int32
  * [num_axes][num_tokens], rows *_axis_stride apart.
  *

@@ -48,10 +48,12 @@
 // have one stride, so a K or V tile of any page size is one matrix operand.
 //
 // Bound by: the serial chain scores -> exponentials -> P -> product of chunks
-// (tensor pipe 60 %, MUFU 61 % busy; 4,096 tokens of 32 / 8 heads of 128 over
-// 131,072 keys, bf16: 6.9 ms = 1,250 TFLOP/s, 9.0 ms with the V fog, where the
-// power cap holds the clock near 1.75 GHz), HBM for decodes (28 of 1k-16k keys:
-// 6.0 TB/s, every key read once), launches and the plan for the smallest (17 us).
+// (2,048 tokens of 32 / 8 heads of 128 over 32,768 keys, bf16: tensor pipe 60 %,
+// MUFU 61 % busy under ncu, 0.99 ms; 4,096 over 131,072: 6.8-7.1 ms = 1,220-1,270
+// TFLOP/s in the first launches, 7.65 ms = 1,130 in a row of them, 9.0 ms with the
+// V fog, where the power cap holds the clock near 1.75 GHz), HBM for decodes (28
+// of 1k-16k keys, 0.69 GB of K/V: 141 us = 4.9 TB/s; 28 of 1.04 GB: 6.0 TB/s under
+// ncu, every key read once), launches and the plan for the smallest (17 us).
 //
 // Every mbarrier wait is bounded; on a timeout all warps still reach the final
 // barrier and the TMEM is freed.

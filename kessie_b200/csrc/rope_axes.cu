@@ -12,9 +12,11 @@
 // by up to 0.06 rad.  The host stores F_d = frac(f_d / 2 pi) as a 64-bit
 // fixed-point fraction of a turn; position * F_d mod 2^64 is the angle's
 // fraction of a turn, off by less than |position| * 2^-64 turns, with no range
-// reduction, and its top 32 bits are kept.  For fp32 rows sincospif takes it
-// from there (~1e-7); for 16-bit rows the hardware sine and cosine on [-pi, pi]
-// do (absolute error below 5e-7, against 2^-12 of the stored rounding).
+// reduction, and its top 32 bits are kept.  As a float a fraction is off by at
+// most 2^-25 half turns (9.4e-8 rad).  For fp32 rows sincospif takes it from there
+// (2 ulp); for 16-bit rows the hardware sine and cosine on [-pi, pi] do: 4.2e-7 at
+// most, and 3.0e-7 for the argument (that rounding, the one of the product with
+// pi and of pi itself): below 7.2e-7, against 2^-11 of the stored rounding.
 //
 // HBM-bound: every row is read and written once (16 bytes a thread and access).
 // A thread owns one vector pair (VEC neighbouring frequencies) of one token and

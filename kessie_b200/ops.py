@@ -690,7 +690,9 @@ def rope_axes_remap(k: torch.Tensor, orig_positions, target_positions, sections:
     dimensions; in blocks, or interleaved over the frequencies (d to axis
     d % axes while d < axes * sections[axis], else to the first).  With
     orig_positions None the keys are rotated from position 0.  Angles are
-    exact to fp32 at any int32 position."""
+    fixed-point fractions of a turn, exact to 2^-31 of it at any int32 position;
+    their sine and cosine are good to 3e-7 for fp32 rows, 7.2e-7 for 16-bit
+    rows."""
     out = k if out is None else out
     index = _one_device("rope_axes_remap", k, out)
     if index != torch.cuda.current_device() or stream is not None:
