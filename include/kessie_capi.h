@@ -254,6 +254,8 @@ int kessie_build_fog_weights_v2(float* out, int seq_len, int clear_start, float 
  *   f32 (q, caches and out all fp32) runs every product in fp32 on the CUDA
  *   cores, for the reference's fp32 path at its 1e-4 bar; the additive-bias
  *   and context-parallel forms below take f16 / bf16 only.
+ *   A row that sees no key is 0 (m = -inf, l = 0); one whose scores are NaN
+ *   (its query is not finite) is NaN (l = NaN), through the combine too.
  * workspace: kessie_paged_fog_decode_workspace_size(...) bytes.
  * f16 / bf16 decodes are programmatic dependent launches: when the last such
  * launch of this library on the same (device, stream) wrote none of q, the

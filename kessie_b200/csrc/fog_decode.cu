@@ -286,35 +286,35 @@ __device__ void merge_and_emit(const DecodeParams& p, int g, int first, int K, i
         float L = 0.f, acc[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = 0.f;
-        if (M != -INFINITY) {
-            for (int kb = 0; kb < K; kb += 32) {
-                const int k = kb + lane;
-                float w = 0.f;
-                if (k < K) {
-                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((size_t)(first + k + g) * p.G + q) * 2));
-                    w = ml.y * exp2f(ml.x - M);
-                }
-                L += w;
-                const int n = min(32, K - kb);
-                const float* base = p.part_o + ((size_t)(first + kb + g) * p.G + q) * D + lane * E;
+        // a row of NaN scores has a NaN l beside m = -inf (maxima pass NaN over): its weight 0 * l keeps it NaN
+        const float base_m = M == -INFINITY ? 0.f : M;
+        for (int kb = 0; kb < K; kb += 32) {
+            const int k = kb + lane;
+            float w = 0.f;
+            if (k < K) {
+                const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((size_t)(first + k + g) * p.G + q) * 2));
+                w = ml.y * exp2f(ml.x - base_m);
+            }
+            L += w;
+            const int n = min(32, K - kb);
+            const float* base = p.part_o + ((size_t)(first + kb + g) * p.G + q) * D + lane * E;
 #pragma unroll 8
-                for (int j = 0; j < n; ++j) {
-                    const float wj = __shfl_sync(0xffffffffu, w, j);
-                    const float* pc = base + (size_t)j * sstride;
-                    if (E == 4) {
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(pc));
-                        acc[0] += wj * x.x; acc[1] += wj * x.y; acc[2] += wj * x.z; acc[3] += wj * x.w;
-                    } else {
-                        const float2 x = __ldcg(reinterpret_cast<const float2*>(pc));
-                        acc[0] += wj * x.x; acc[1] += wj * x.y;
-                    }
+            for (int j = 0; j < n; ++j) {
+                const float wj = __shfl_sync(0xffffffffu, w, j);
+                const float* pc = base + (size_t)j * sstride;
+                if (E == 4) {
+                    const float4 x = __ldcg(reinterpret_cast<const float4*>(pc));
+                    acc[0] += wj * x.x; acc[1] += wj * x.y; acc[2] += wj * x.z; acc[3] += wj * x.w;
+                } else {
+                    const float2 x = __ldcg(reinterpret_cast<const float2*>(pc));
+                    acc[0] += wj * x.x; acc[1] += wj * x.y;
                 }
             }
-            L = warp_sum(L);
         }
+        L = warp_sum(L);
         float o[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = L > 0.f ? acc[e] / L : 0.f;
+        for (int e = 0; e < E; ++e) o[e] = L == 0.f ? 0.f : acc[e] / L;
         emit_row<D, BF16>(p, b * p.Hq + hk * p.G + q, lane, o, M, L);
     }
 }
@@ -787,8 +787,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) fog_decode_kernel(c
                         const float L = l[nt][j];
 #pragma unroll
                         for (int mt = 0; mt < D / 16; ++mt) {
-                            po[mt * 16 + g8] = L > 0.f ? acc[nt][mt][j] / L : 0.f;
-                            po[mt * 16 + g8 + 8] = L > 0.f ? acc[nt][mt][2 + j] / L : 0.f;
+                            po[mt * 16 + g8] = L == 0.f ? 0.f : acc[nt][mt][j] / L;
+                            po[mt * 16 + g8 + 8] = L == 0.f ? 0.f : acc[nt][mt][2 + j] / L;
                         }
                         if (g8 == 0) *reinterpret_cast<float2*>(pm) = make_float2(m[nt][j], L);
                     }
@@ -898,21 +898,20 @@ __global__ void __launch_bounds__(128) cp_combine_kernel(const CpCombineParams a
 #pragma unroll
         for (int s = 0; s < kCpMaxRanks; ++s)
             if (s < world) M = fmaxf(M, ms[s]);
-        if (M != -INFINITY) {
+        const float base_m = M == -INFINITY ? 0.f : M;       // a NaN l beside m = -inf stays NaN (merge_and_emit)
 #pragma unroll
-            for (int s = 0; s < kCpMaxRanks; ++s) {
-                if (s < world) {
-                    const float ws = ls[s] * exp2f(ms[s] - M);
-                    L += ws;
+        for (int s = 0; s < kCpMaxRanks; ++s) {
+            if (s < world) {
+                const float ws = ls[s] * exp2f(ms[s] - base_m);
+                L += ws;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] += ws * x[s][e];
-                }
+                for (int e = 0; e < E; ++e) acc[e] += ws * x[s][e];
             }
         }
     }
     float o[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = L > 0.f ? acc[e] / L : 0.f;
+    for (int e = 0; e < E; ++e) o[e] = L == 0.f ? 0.f : acc[e] / L;
     if (!ok) { M = -INFINITY; L = 0.f; }
     if (a.out) store_out_row<BF16>(a.out, (int64_t)row * D + lane * E, o, E);
     if (a.out_part) {
@@ -935,15 +934,14 @@ __global__ void lse_combine_kernel(const float* __restrict__ parts, int S, int64
     float M = -INFINITY;
     for (int s = 0; s < S; ++s) M = fmaxf(M, parts[s * sstride + (int64_t)row * (D + 2) + D]);
     float L = 0.f, O = 0.f;
-    if (M != -INFINITY) {
-        for (int s = 0; s < S; ++s) {
-            const float* pr = parts + s * sstride + (int64_t)row * (D + 2);
-            const float w = pr[D + 1] * __expf(pr[D] - M);
-            L += w;
-            O += w * pr[d];
-        }
+    const float base_m = M == -INFINITY ? 0.f : M;           // a NaN l beside m = -inf stays NaN (merge_and_emit)
+    for (int s = 0; s < S; ++s) {
+        const float* pr = parts + s * sstride + (int64_t)row * (D + 2);
+        const float w = pr[D + 1] * __expf(pr[D] - base_m);
+        L += w;
+        O += w == 0.f ? 0.f : w * pr[d];
     }
-    const float o = L > 0.f ? O / L : 0.f;
+    const float o = L == 0.f ? 0.f : O / L;
     if (out) out[(int64_t)row * D + d] = from_f32<T>(o);
     if (out_part) {
         out_part[(int64_t)row * (D + 2) + d] = o;

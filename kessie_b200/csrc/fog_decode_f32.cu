@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(kT, 1) fog_decode_f32_kernel(const DecodeF32Ar
             const int g = i / D, d = i - g * D;
             const float M = sML[g * 2], L = sML[g * 2 + 1];
             float o = 0.f;
-            if (L > 0.f) {
+            if (L != 0.f) {                  // NaN scores: L is NaN, and so is the row
                 for (int w2 = 0; w2 < kW; ++w2) o = fmaf(warp_area(w2)[2 * GP + g * D + d], sSC[w2 * GP + g], o);
                 o /= L;
             }
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(kT, 1) fog_decode_f32_kernel(const DecodeF32Ar
         const int g = i / D, d = i - g * D;
         const float M = sML[g * 2], L = sML[g * 2 + 1];
         float o = 0.f;
-        if (L > 0.f) {
+        if (L != 0.f) {
             for (int w2 = 0; w2 < kW; ++w2) o = fmaf(warp_area(w2)[2 * GP + g * D + d], sSC[w2 * GP + g], o);
             o /= L;
         }
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(kT, 1) fog_decode_f32_kernel(const DecodeF32Ar
         float L = 0.f;
         for (int s2 = lane; s2 < S; s2 += 32) {
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((size_t)(grp * S + s2) * G + g) * 2));
-            const float sc = ml.x == -INFINITY ? 0.f : ml.y * exp2f(ml.x - M);
+            const float sc = ml.y * (ml.x == -INFINITY ? 0.f : exp2f(ml.x - M));      // NaN for a NaN l
             ssc[s2 * GP + g] = sc;
             L += sc;
         }
@@ -605,7 +605,7 @@ __global__ void __launch_bounds__(kT, 1) fog_decode_f32_kernel(const DecodeF32Ar
         const int g = i / D, d = i - g * D;
         const float M = sML[g * 2], L = sML[g * 2 + 1];
         float o = 0.f;
-        if (L > 0.f) {
+        if (L != 0.f) {
             for (int s2 = 0; s2 < S; ++s2) {
                 const float sc = ssc[s2 * GP + g];
                 if (sc != 0.f) o = fmaf(__ldcg(p.part_o + ((size_t)(grp * S + s2) * G + g) * D + d), sc, o);
