@@ -270,7 +270,7 @@ class KeSSieAttentionImpl:
         capacity = bt.shape[1] * key_cache.shape[1]
         if (getattr(md, "max_seq_len", None) or 0) > capacity:
             self._check_lengths(md, capacity)
-        for run in self._launches(md, B, capacity, key_cache.shape[1]):
+        for run in self._launches(md, B, capacity, key_cache.shape[1], out):
             if run.decodes:
                 rows, reqs = slice(run.row, run.row + run.end - run.first), slice(run.first, run.end)
                 ops.paged_fog_decode(q[rows], key_cache, value_cache, bt[reqs], sl[reqs], out=out[rows], **kw)
@@ -281,7 +281,7 @@ class KeSSieAttentionImpl:
                                      **kw)
         return output
 
-    def _launches(self, md, B, capacity, page_size):
+    def _launches(self, md, B, capacity, page_size, out):
         """The calls of a mixed step of B requests: all of them in one
         ragged-chunk call, or the decodes apart in the paged decode.  The
         latter takes the metadata builder's host copy of the offsets; a capture
@@ -292,7 +292,9 @@ class KeSSieAttentionImpl:
             return whole
         tiles = sum(r.end - r.first for r in runs if r.decodes) * self._num_kv_heads
         sms = torch.cuda.get_device_properties(md.seq_lens.device).multi_processor_count
-        if tiles < _SPLIT_TILES * sms or page_size > 256 or tiles * (capacity // 16) > 1 << 30:  # the decode's limits
+        if tiles < _SPLIT_TILES * sms:
+            return whole
+        if page_size > 256 or tiles * (capacity // 16) > 1 << 30 or not out.is_contiguous():      # the decode's limits
             return whole
         return runs
 
@@ -308,8 +310,8 @@ except Exception:                                      # pragma: no cover - depe
 if HAS_VLLM:
     class KeSSieAttentionBackend(_FlashAttentionBackend):
         """FlashAttention backend whose implementation applies the fog
-        (kessie_attention.py:228-260); metadata, builder and cache layout are
-        FlashAttention's."""
+        (kessie_attention.py:228-260); metadata and cache layout are
+        FlashAttention's, and so is the builder but for a mixed step's runs."""
 
         @classmethod
         def _get_original(cls):

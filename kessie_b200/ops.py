@@ -331,6 +331,9 @@ def paged_fog_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     B, Hq, D = q.shape
     if want_out and out is None:
         out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
+    elif want_out and (out.numel() != q.numel() or out.dtype != q.dtype or out.device != q.device
+                       or not out.is_contiguous()):
+        raise ValueError("paged_fog_decode: out must be contiguous, of q's dtype, device and size")
     lib, args, ws, keep = _decode_args(q, k_cache, v_cache, block_table, seq_lens, clear_start, fog_alpha,
                                        fog_weights, window_size, sm_scale, kv_pos_offset, q_positions, max_seq_len, ws)
     if bias is not None:

@@ -1,4 +1,5 @@
-"""GPU: the decode's scratch needs no initialisation, whatever it held before.
+"""GPU: the decode's scratch needs no initialisation, whatever it held before;
+outputs that it cannot write are refused.
 
 The arrival counters in it are told from leftovers by a tag of the launch, so
 a process's first launches are tried on scratch full of 64-bit words whose
@@ -50,3 +51,21 @@ def test_decode_on_scratch_full_of_small_numbers():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", CODE], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stderr[-2000:]
+
+
+def test_decode_refuses_outputs_it_would_write_past():
+    """The rows are written next to one another: an output with gaps between
+    them, of another type or another size is not what the kernel writes."""
+    from kessie_b200 import ops
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    kv = torch.randn(4, 16, 2, 2, 128, device="cuda").half()
+    table, lens = torch.arange(4, device="cuda").int().view(2, 2), torch.tensor([20, 32], device="cuda").int()
+    q = torch.randn(2, 8, 128, device="cuda").half()
+    wide = torch.zeros(2, 10, 128, device="cuda", dtype=torch.float16)
+    for out in (wide[:, 1:9], torch.zeros(2, 8, 128, device="cuda"), wide[:1, :8], torch.zeros(2, 8, 128).half()):
+        with pytest.raises(ValueError, match="out must be"):
+            ops.paged_fog_decode(q, kv[:, :, 0], kv[:, :, 1], table, lens, out=out)
+    flat = torch.zeros(2, 8 * 128, device="cuda", dtype=torch.float16)
+    ops.paged_fog_decode(q, kv[:, :, 0], kv[:, :, 1], table, lens, out=flat)
+    assert torch.equal(flat.view(2, 8, 128), ops.paged_fog_decode(q, kv[:, :, 0], kv[:, :, 1], table, lens))
