@@ -162,16 +162,17 @@ class QueryRun(NamedTuple):
     decodes: bool
 
 
-def query_runs(starts: Sequence[int]) -> Tuple[QueryRun, ...]:
-    """The runs of a step, from the offsets of its requests' tokens."""
-    runs = []
-    for i in range(len(starts) - 1):
-        one = starts[i + 1] - starts[i] == 1
-        if runs and runs[-1].decodes == one:
-            runs[-1] = runs[-1]._replace(end=i + 1)
-        else:
-            runs.append(QueryRun(i, i + 1, starts[i], one))
-    return tuple(runs)
+def query_runs(starts: Sequence[int], most: Optional[int] = None) -> Tuple[QueryRun, ...]:
+    """The runs of a step, from the offsets of its requests' tokens (on the
+    host); none of them where there are more than `most`."""
+    starts = torch.as_tensor(starts, device="cpu")
+    one = starts.diff() == 1
+    if one.numel() == 0:
+        return ()
+    firsts = [0] + ((one[1:] != one[:-1]).nonzero().flatten() + 1).tolist()
+    if most is not None and len(firsts) > most:
+        return ()
+    return tuple(QueryRun(f, e, int(starts[f]), bool(one[f])) for f, e in zip(firsts, firsts[1:] + [one.numel()]))
 
 
 # A mixed step's decodes go to the paged decode, apart from its chunks, when there is one run of each and the decodes
@@ -337,7 +338,7 @@ if HAS_VLLM:
             md = super().build(common_prefix_len, common_attn_metadata, fast_build)
             starts = getattr(common_attn_metadata, "query_start_loc_cpu", None)
             if starts is not None and common_attn_metadata.max_query_len > 1:
-                md.query_runs = query_runs(starts.tolist())
+                md.query_runs = query_runs(starts, 2)           # of more the attention makes no use
             return md
 else:
     class KeSSieAttentionBackend:                      # pragma: no cover

@@ -16,6 +16,7 @@ def test_query_runs(q_lens, want):
     from kessie_b200.kessie_attention import query_runs
     starts = [sum(q_lens[:i]) for i in range(len(q_lens) + 1)]
     assert [tuple(r) for r in query_runs(starts)] == want
+    assert [tuple(r) for r in query_runs(starts, 2)] == (want if len(want) <= 2 else [])
 
 
 def test_builder_adds_the_runs_to_flash_attentions_metadata(monkeypatch):
